@@ -285,6 +285,146 @@ int rai_rope_apply_dev(float *heads, size_t num_heads, size_t head_dim, const fl
 int rai_attention_head_dev(float *out, const float *q, const float *k, const float *v, size_t pos,
                            size_t head_dim, float scale, void *stream);
 
+/* ------------------------------------------------ paged KV cache (device) -- */
+/* No counterpart in the reference, whose cache holds one sequence
+ * (kv_cache.rs).  Several sequences share a pool of fixed-size pages; each has
+ * a table of page ids, and position p of a sequence lies in slot p % page_size
+ * of page table[p / page_size].  Which page belongs to whom is the caller's to
+ * decide: the calls below fill, read, fork and move the pages.
+ *
+ * All pointers in the structures are device pointers, and so are the calls'
+ * arrays; the structures themselves are host memory, read during the call.
+ * The calls are asynchronous on `stream`, allocate nothing, keep nothing
+ * between calls and may be captured into a graph.  Entries of device arrays
+ * cannot fail a call; they are bounded instead: a page id outside 0..pages-1
+ * is a page that is not there (nothing is read from it or written to it, and
+ * its keys are not seen), row starts and lengths are cut to the bounds given
+ * with them. */
+typedef enum rai_cache_type { RAI_CACHE_F32 = 0, RAI_CACHE_F16 = 1, RAI_CACHE_BF16 = 2 } rai_cache_type;
+
+/* The pool: k [layers][pages][kv_heads][page_size][head_dim] and
+ * v [layers][pages][kv_heads][head_dim][page_size] (a head's values lie
+ * dimension by dimension, as in the model's own cache) of `type`, 16-byte
+ * aligned.  page_size is a power of two from 16 to 1024, head_dim a multiple of
+ * 8 up to 256. */
+typedef struct rai_pages {
+  void *k, *v;
+  size_t layers, pages, page_size, kv_heads, head_dim;
+  int type; /* rai_cache_type */
+} rai_pages;
+
+/* A batch of sequences and their new tokens.  Rows q_start[s]..q_start[s+1]-1
+ * (q_start ascending) are the new tokens of sequence s, at the last positions
+ * of its kv_len[s] ones: row q_start[s] + j is position kv_len[s] -
+ * (q_start[s+1] - q_start[s]) + j.  Rows in front of the first sequence and
+ * behind the last are nobody's: they are not touched.  max_q bounds the new
+ * tokens of a sequence and max_kv its length (they size the launch; lengths
+ * past them or past the table are cut). */
+typedef struct rai_page_batch {
+  const int32_t *tables; /* [seqs][table_stride] page ids */
+  size_t table_stride;
+  const int32_t *q_start; /* [seqs + 1] */
+  const int32_t *kv_len;  /* [seqs] */
+  size_t seqs, tokens, max_q, max_kv;
+} rai_page_batch;
+
+/* Rotary positions: pair i of the first rot_dim dimensions - (i, i + rot_dim/2),
+ * or (2i, 2i + 1) when interleaved - turns by position * inv_freq[i] (device,
+ * [rot_dim / 2], f64; the angle is reduced in f64) and is multiplied by `gain`;
+ * the other dimensions pass. */
+typedef struct rai_rope {
+  const double *inv_freq;
+  size_t rot_dim;
+  int interleaved;
+  float gain;
+} rai_rope;
+
+typedef enum rai_rope_scaling {
+  RAI_ROPE_NONE = 0,
+  RAI_ROPE_LINEAR = 1, /* every frequency divided by factor */
+  RAI_ROPE_LLAMA3 = 2, /* those that turn less than low_freq times over trained_context divided, those
+                          that turn more than high_freq times kept, blended between */
+  RAI_ROPE_YARN = 3    /* the same blended by pair index (low_freq, high_freq: 1 and 32 turns), and
+                          the gain 0.1 ln(factor) + 1 */
+} rai_rope_scaling;
+
+/* Host only: the inverse frequencies theta^(-2i / rot_dim), i < rot_dim / 2, under
+ * a scaling, and the gain that goes with it (1 except for YaRN).  factor >= 1,
+ * trained_context > 0 and 0 < low_freq < high_freq where the scaling reads them. */
+int rai_rope_frequencies(int scaling, double theta, size_t rot_dim, double factor, double trained_context,
+                         double low_freq, double high_freq, double *inv_freq, float *gain);
+
+/* Rotates the batch's queries and keys and puts keys and values into `layer` of
+ * their sequences' pages, rounded once (to nearest, ties to even) to the cache's
+ * type.  q, k and v hold a row per token, rows q_stride, k_stride and v_stride
+ * floats apart ([heads][head_dim] or [kv_heads][head_dim] each); q_out rows lie
+ * q_out_stride apart and may be q itself (same stride).  heads == 0: no queries
+ * (q and q_out are not read).  rope == NULL: nothing turns.  Rows whose position
+ * is negative or has no page are rotated and not stored.  Two rows of one batch
+ * at the same slot: one of them is kept. */
+int rai_paged_store_dev(const rai_pages *pages, size_t layer, const rai_page_batch *batch, const rai_rope *rope,
+                        float *q_out, size_t q_out_stride, const float *q, size_t q_stride, size_t heads,
+                        const float *k, size_t k_stride, const float *v, size_t v_stride, void *stream);
+
+/* score = q . k * scale; with softcap > 0: softcap * tanh(score / softcap); with
+ * slopes (device, [heads]): minus slopes[h] * (row's position - key's position).
+ * window > 0: a row sees the last `window` positions up to its own. */
+typedef struct rai_attention_options {
+  float scale, softcap;
+  size_t window;
+  const float *slopes;
+} rai_attention_options;
+
+/* Causal attention of the batch's rows over `layer` of their sequences' pages
+ * (keys and values of the rows themselves are in the pages: rai_paged_store_dev
+ * first): out row = sum_j softmax_j(score) v_j over the positions it sees, heads /
+ * kv_heads query heads on each kv head.  f32 accuracy for every cache type.  A row
+ * that sees nothing becomes zeros.  What a row does not see does not reach it,
+ * NaN and infinities included.
+ * work: scratch of the call (16-byte aligned), with which long contexts of few
+ * rows are split over the chip; rai_paged_attention_workspace gives the size that
+ * the call can use, less (or none) means fewer splits.  Calls that overlap in time
+ * need scratch of their own.  The same arguments give the same bits. */
+int rai_paged_attention_workspace(size_t heads, const rai_pages *pages, const rai_page_batch *batch,
+                                  const rai_attention_options *options, size_t *bytes);
+int rai_paged_attention_dev(float *out, size_t out_stride, const float *q, size_t q_stride, size_t heads,
+                            const rai_pages *pages, size_t layer, const rai_page_batch *batch,
+                            const rai_attention_options *options, void *work, size_t work_bytes, void *stream);
+
+/* n sequences that go on from parents (a beam step, several samples of one
+ * prompt): row i of tables_out becomes row parent[i] of tables, lengths_out[i] its
+ * length.  Full pages are shared.  The last page, when part filled, stays with the
+ * lowest i of a parent; every later child gets page fresh[i] in its place, with the
+ * contents copied in all layers, and used[i] = 1 (else 0).  tables [seqs] and
+ * tables_out [n] have rows of table_stride ids and must not overlap; the fresh pages
+ * must be distinct and nobody's.  A parent outside 0..seqs-1: lengths_out 0, a table
+ * row of -1.  Without a valid fresh[i] the entry becomes -1. */
+int rai_paged_fork_dev(const rai_pages *pages, const int32_t *tables, size_t table_stride, const int32_t *lengths,
+                       size_t seqs, const int32_t *parent, const int32_t *fresh, size_t n, int32_t *tables_out,
+                       int32_t *lengths_out, int32_t *used, void *stream);
+
+/* Moves n pages: page src[i] is copied to dst[i] in all layers, and each of the
+ * `entries` ids of `tables` (may be NULL) that names src[i] names dst[i] afterwards.
+ * src are distinct, dst are distinct and none of src (a copy goes to a free page).
+ * Pairs with an id outside the pool are left out. */
+int rai_paged_move_dev(const rai_pages *pages, const int32_t *src, const int32_t *dst, size_t n, int32_t *tables,
+                       size_t entries, void *stream);
+
+/* Beam search's selection: logits [groups * beams] rows of vocab, `stride` floats
+ * apart; scores [groups * beams].  A candidate (beam, token) scores scores[beam] +
+ * log softmax(logits row)[token]; each group's best `take` go to parent (the row:
+ * group * beams + beam, what rai_paged_fork_dev takes), token and score
+ * [groups][take], best first, equal ones by beam, then logit, then token.  done (may be NULL)
+ * [groups * beams]: a finished beam's only candidate is end_token at its present
+ * score.  Scores are summed and compared in f64.  NaN logits count as -inf; a row
+ * without a finite log-sum (all -inf, or +inf) and beams at -inf or NaN have no
+ * candidates, and neither has a token at -inf; places past the last candidate
+ * become -1, -1, -inf.  beams <= 64, take <= 64. */
+int rai_beam_select_workspace(size_t vocab, size_t groups, size_t beams, size_t take, size_t *bytes);
+int rai_beam_select_dev(const float *logits, size_t stride, size_t vocab, const float *scores, const uint8_t *done,
+                        int32_t end_token, size_t groups, size_t beams, size_t take, int32_t *parent,
+                        int32_t *token, float *score, void *work, size_t work_bytes, void *stream);
+
 /* -------------------------------------------- draft-model speculation -- */
 /* SpeculativeDecoder::new (speculative.rs:79-110): both models must share
  * the vocabulary; the context is the smaller of both windows and max_ctx. */

@@ -49,6 +49,32 @@ class QLinear(ctypes.Structure):
                 ("group_size", c_size_t)]
 
 
+CACHE_F32, CACHE_F16, CACHE_BF16 = 0, 1, 2
+ROPE_NONE, ROPE_LINEAR, ROPE_LLAMA3, ROPE_YARN = 0, 1, 2, 3
+
+
+class Pages(ctypes.Structure):
+    """rai_pages: the pool of a paged KV cache, device pointers."""
+    _fields_ = [("k", c_void_p), ("v", c_void_p), ("layers", c_size_t), ("pages", c_size_t),
+                ("page_size", c_size_t), ("kv_heads", c_size_t), ("head_dim", c_size_t), ("type", c_int)]
+
+
+class PageBatch(ctypes.Structure):
+    """rai_page_batch: a batch of sequences over the pages, device pointers."""
+    _fields_ = [("tables", c_void_p), ("table_stride", c_size_t), ("q_start", c_void_p), ("kv_len", c_void_p),
+                ("seqs", c_size_t), ("tokens", c_size_t), ("max_q", c_size_t), ("max_kv", c_size_t)]
+
+
+class Rope(ctypes.Structure):
+    """rai_rope: rotary positions from device inverse frequencies (rope_frequencies)."""
+    _fields_ = [("inv_freq", c_void_p), ("rot_dim", c_size_t), ("interleaved", c_int), ("gain", c_float)]
+
+
+class AttentionOptions(ctypes.Structure):
+    """rai_attention_options: scale, score cap (0 = off), window (0 = off), per-head slopes (device, or None)."""
+    _fields_ = [("scale", c_float), ("softcap", c_float), ("window", c_size_t), ("slopes", c_void_p)]
+
+
 class ModelConfig(ctypes.Structure):
     _fields_ = [(n, c_uint32) for n in (
         "hidden_size", "num_layers", "num_heads", "num_kv_heads", "head_dim",
@@ -138,6 +164,18 @@ def lib():
         "rai_silu_mul_dev": (c_int, [P, P, S, S, P]),
         "rai_rope_apply_dev": (c_int, [P, S, S, P, P, P]),
         "rai_attention_head_dev": (c_int, [P, P, P, P, S, S, c_float, P]),
+        "rai_rope_frequencies": (c_int, [c_int, c_double, S, c_double, c_double, c_double, c_double, P,
+                                         POINTER(c_float)]),
+        "rai_paged_store_dev": (c_int, [POINTER(Pages), S, POINTER(PageBatch), POINTER(Rope), P, S, P, S, S, P, S,
+                                        P, S, P]),
+        "rai_paged_attention_workspace": (c_int, [S, POINTER(Pages), POINTER(PageBatch), POINTER(AttentionOptions),
+                                                  POINTER(c_size_t)]),
+        "rai_paged_attention_dev": (c_int, [P, S, P, S, S, POINTER(Pages), S, POINTER(PageBatch),
+                                            POINTER(AttentionOptions), P, S, P]),
+        "rai_paged_fork_dev": (c_int, [POINTER(Pages), P, S, P, S, P, P, S, P, P, P, P]),
+        "rai_paged_move_dev": (c_int, [POINTER(Pages), P, P, S, P, S, P]),
+        "rai_beam_select_workspace": (c_int, [S, S, S, S, POINTER(c_size_t)]),
+        "rai_beam_select_dev": (c_int, [P, S, S, P, P, ctypes.c_int32, S, S, S, P, P, P, P, S, P]),
         "rai_find_ngram_draft": (c_int, [P, S, S, S, S, POINTER(_LookupMatch), POINTER(c_int)]),
         "rai_lookup_create": (c_int, [P, S, POINTER(c_void_p)]),
         "rai_lookup_free": (None, [P]),
@@ -257,6 +295,30 @@ class DeviceArray:
 
 
 # ---------------------------------------------------------------- kernels --
+
+def rope_frequencies(scaling: int, theta: float, rot_dim: int, factor: float = 1.0, trained_context: float = 8192.0,
+                     low_freq: float = 1.0, high_freq: float = 4.0) -> tuple[np.ndarray, float]:
+    """rai_rope_frequencies: (inverse frequencies [rot_dim / 2] in f64, gain) of a rotary scaling."""
+    inv, gain = np.zeros(rot_dim // 2, np.float64), c_float()
+    _check(lib().rai_rope_frequencies(scaling, theta, rot_dim, factor, trained_context, low_freq, high_freq,
+                                      _ptr(inv), ctypes.byref(gain)))
+    return inv, gain.value
+
+
+def attention_workspace(heads: int, pages: Pages, batch: PageBatch, options: AttentionOptions) -> int:
+    """rai_paged_attention_workspace: bytes of scratch that the call can use."""
+    n = c_size_t()
+    _check(lib().rai_paged_attention_workspace(heads, ctypes.byref(pages), ctypes.byref(batch),
+                                               ctypes.byref(options), ctypes.byref(n)))
+    return n.value
+
+
+def beam_workspace(vocab: int, groups: int, beams: int, take: int) -> int:
+    """rai_beam_select_workspace: bytes of scratch that the call needs."""
+    n = c_size_t()
+    _check(lib().rai_beam_select_workspace(vocab, groups, beams, take, ctypes.byref(n)))
+    return n.value
+
 
 def w4a8_matmul(nibbles, params, x, rows: int, cols: int, num_tokens: int,
                 group_size: int) -> np.ndarray:

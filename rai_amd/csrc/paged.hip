@@ -1,0 +1,405 @@
+// The paged KV cache: what fills it (rotary positions and the store), what forks
+// and moves its pages, and the checks of its entry points.  The attention over it
+// is in paged_attn.hip.
+#include "paged.h"
+
+#include <algorithm>
+#include <cmath>
+#include <cstring>
+
+namespace rai {
+
+namespace {
+
+constexpr int kMaxHd = 256;
+
+// ------------------------------------------------------------------- store --
+
+struct RopeView {
+  const double *inv;
+  int rot;
+  bool inter;
+  float gain;
+};
+
+struct StoreArgs {
+  float *q_out;
+  const float *q, *k, *v;
+  size_t qo_ld, q_ld, k_ld, v_ld;
+  int heads;
+  RopeView rope;
+};
+
+// cos and sin of pos * inv, both times gain: the product and its reduction to
+// -pi..pi in f64 (an f32 angle of a far position is off by more than the rotation
+// may be), the functions of the reduced angle in f32.
+__device__ __forceinline__ void rope_angle(int pos, double inv, float gain, float &c, float &s) {
+  const double a = (double)pos * inv;
+  const double n = rint(a * 0.15915494309189535);
+  double r = fma(-n, 6.283185307179586, a);
+  r = fma(-n, 2.4492935982947064e-16, r);
+  sincosf((float)r, &s, &c);
+  c *= gain;
+  s *= gain;
+}
+
+// The pair (e0, e1) of rotated pair i.
+__device__ __forceinline__ void pair_of(const RopeView &r, int i, int &e0, int &e1) {
+  e0 = r.inter ? 2 * i : i;
+  e1 = r.inter ? 2 * i + 1 : i + r.rot / 2;
+}
+
+// A block per row: queries and keys pair by pair, values element by element.
+template <class T>
+__global__ __launch_bounds__(256) void k_store(StoreArgs a, LayerView<T> kv, BatchView b) {
+  const SeqSpan sp = seq_span(b, blockIdx.y);
+  const int j = blockIdx.x;
+  if (j >= sp.nq) return;
+  __shared__ float cs[kMaxHd / 2], sn[kMaxHd / 2];
+  const int row = sp.q0 + j, pos = sp.n - sp.nq + j, half = a.rope.rot / 2;
+  for (int i = threadIdx.x; i < half; i += 256) rope_angle(pos, a.rope.inv[i], a.rope.gain, cs[i], sn[i]);
+  __syncthreads();
+  const int hd = kv.hd, units = half + (hd - a.rope.rot);  // of a head: pairs, then single elements
+  for (int u = threadIdx.x; u < a.heads * units; u += 256) {
+    const int h = u / units, i = u % units;
+    const float *x = a.q + (size_t)row * a.q_ld + (size_t)h * hd;
+    float *o = a.q_out + (size_t)row * a.qo_ld + (size_t)h * hd;
+    if (i < half) {
+      int e0, e1;
+      pair_of(a.rope, i, e0, e1);
+      const float x0 = x[e0], x1 = x[e1];
+      o[e0] = x0 * cs[i] - x1 * sn[i];
+      o[e1] = x1 * cs[i] + x0 * sn[i];
+    } else {
+      o[a.rope.rot + i - half] = x[a.rope.rot + i - half];
+    }
+  }
+  if (pos < 0) return;
+  const int page = page_of(b.tables + (size_t)blockIdx.y * b.stride, pos, kv.shift, kv.pages);
+  if (page < 0) return;
+  const int slot = pos & ((1 << kv.shift) - 1);
+  for (int u = threadIdx.x; u < kv.nkv * units; u += 256) {
+    const int h = u / units, i = u % units;
+    const float *x = a.k + (size_t)row * a.k_ld + (size_t)h * hd;
+    T *o = kv.k + key_at(page, h, slot, kv.nkv, hd, kv.shift);
+    if (i < half) {
+      int e0, e1;
+      pair_of(a.rope, i, e0, e1);
+      const float x0 = x[e0], x1 = x[e1];
+      o[e0] = from_f32<T>(x0 * cs[i] - x1 * sn[i]);
+      o[e1] = from_f32<T>(x1 * cs[i] + x0 * sn[i]);
+    } else {
+      o[a.rope.rot + i - half] = from_f32<T>(x[a.rope.rot + i - half]);
+    }
+  }
+  for (int u = threadIdx.x; u < kv.nkv * hd; u += 256) {
+    const int h = u / hd, d = u % hd;
+    kv.v[value_at(page, h, slot, kv.nkv, hd, kv.shift) + ((size_t)d << kv.shift)] =
+        from_f32<T>(a.v[(size_t)row * a.v_ld + u]);
+  }
+}
+
+template <class T>
+void launch_store(const StoreArgs &a, const LayerView<T> &kv, const BatchView &b, hipStream_t s) {
+  k_store<T><<<dim3(b.max_q, b.seqs), 256, 0, s>>>(a, kv, b);
+}
+
+// ----------------------------------------------------------- forks and moves --
+
+// The pool as bytes: a page of one layer's keys (or values) is `bytes` long, a
+// multiple of 16.
+struct PoolBytes {
+  uint4 *k, *v;
+  size_t layer_vecs, page_vecs;
+  int layers, pages;
+};
+
+__device__ __forceinline__ void copy_page(const PoolBytes &p, int layer, int src, int dst, int tid, int n) {
+  const size_t base = (size_t)layer * p.layer_vecs;
+  const uint4 *ks = p.k + base + (size_t)src * p.page_vecs, *vs = p.v + base + (size_t)src * p.page_vecs;
+  uint4 *kd = p.k + base + (size_t)dst * p.page_vecs, *vd = p.v + base + (size_t)dst * p.page_vecs;
+  for (size_t i = tid; i < p.page_vecs; i += n) {
+    const uint4 x = ks[i], y = vs[i];
+    kd[i] = x;
+    vd[i] = y;
+  }
+}
+
+// Block (layer, child): layer 0's blocks write the table row too.
+__global__ __launch_bounds__(256) void k_fork(PoolBytes p, const int *tables, size_t stride, const int *lengths,
+                                              int seqs, const int *parent, const int *fresh, int n, int *tables_out,
+                                              int *lengths_out, int *used, int shift) {
+  const int i = blockIdx.y, par = parent[i], tid = threadIdx.x;
+  const bool ok = (unsigned)par < (unsigned)seqs;
+  const size_t most = stride << shift;
+  int len = ok ? max(lengths[par], 0) : 0;
+  if ((size_t)len > most) len = (int)most;
+  int again = 0;
+  for (int j = tid; j < i; j += 256) again |= parent[j] == par;
+  again = __syncthreads_or(again);
+  const bool part = (len & ((1 << shift) - 1)) != 0, take = ok && part && again;
+  const int last = len >> shift;  // the part-filled page's place
+  int f = take ? fresh[i] : -1;
+  if ((unsigned)f >= (unsigned)p.pages) f = -1;
+  if (blockIdx.x == 0) {
+    for (size_t c = tid; c < stride; c += 256) {
+      int id = ok ? tables[(size_t)par * stride + c] : -1;
+      if (take && c == (size_t)last) id = f;
+      tables_out[(size_t)i * stride + c] = id;
+    }
+    if (tid == 0) {
+      lengths_out[i] = len;
+      used[i] = take && f >= 0;
+    }
+  }
+  if (!take || f < 0) return;
+  const int src = tables[(size_t)par * stride + last];
+  if ((unsigned)src >= (unsigned)p.pages) return;
+  copy_page(p, blockIdx.x, src, f, tid, 256);
+}
+
+__global__ __launch_bounds__(256) void k_move(PoolBytes p, const int *src, const int *dst, int n) {
+  const int a = src[blockIdx.y], b = dst[blockIdx.y];
+  if ((unsigned)a >= (unsigned)p.pages || (unsigned)b >= (unsigned)p.pages) return;
+  copy_page(p, blockIdx.x, a, b, threadIdx.x, 256);
+}
+
+__global__ __launch_bounds__(256) void k_rename(const int *src, const int *dst, int n, int pages, int *tables,
+                                                size_t entries) {
+  for (size_t e = (size_t)blockIdx.x * 256 + threadIdx.x; e < entries; e += (size_t)gridDim.x * 256) {
+    const int id = tables[e];
+    for (int i = 0; i < n; ++i)
+      if (src[i] == id && (unsigned)id < (unsigned)pages && (unsigned)dst[i] < (unsigned)pages) {
+        tables[e] = dst[i];
+        break;
+      }
+  }
+}
+
+// ------------------------------------------------------------------ checks --
+
+size_t type_bytes(int type) { return type == RAI_CACHE_F32 ? 4 : 2; }
+
+int page_shift(size_t page_size) {
+  int s = 0;
+  while ((size_t(1) << s) < page_size) ++s;
+  return s;
+}
+
+void check_pages(const rai_pages *p) {
+  if (!p || !p->k || !p->v) fail(RAI_E_ARG, "null argument");
+  if (p->type != RAI_CACHE_F32 && p->type != RAI_CACHE_F16 && p->type != RAI_CACHE_BF16)
+    fail(RAI_E_ARG, "unknown cache type");
+  if (p->page_size < 16 || p->page_size > 1024 || (p->page_size & (p->page_size - 1)))
+    fail(RAI_E_SHAPE, "page_size must be a power of two from 16 to 1024");
+  if (p->head_dim == 0 || p->head_dim % 8 || p->head_dim > kMaxHd)
+    fail(RAI_E_SHAPE, "head_dim must be a multiple of 8 up to 256");
+  if (p->layers == 0 || p->pages == 0 || p->kv_heads == 0) fail(RAI_E_SHAPE, "the pool must not be empty");
+  if (p->layers > 65535 || p->pages > INT32_MAX || p->kv_heads > 65535) fail(RAI_E_SHAPE, "dimensions overflow");
+  if ((uintptr_t)p->k % 16 || (uintptr_t)p->v % 16) fail(RAI_E_ARG, "the pages must be 16-byte aligned");
+}
+
+// Null only where there is nothing to do (no sequences or no rows).
+bool check_batch(const rai_page_batch *b, const rai_pages *p, BatchView *v) {
+  if (!b) fail(RAI_E_ARG, "null argument");
+  if (b->seqs == 0 || b->tokens == 0 || b->max_q == 0) return false;
+  if (!b->tables || !b->q_start || !b->kv_len) fail(RAI_E_ARG, "null argument");
+  if (b->table_stride == 0) fail(RAI_E_SHAPE, "table_stride must be non-zero");
+  if (b->seqs > 65535) fail(RAI_E_SHAPE, "at most 65535 sequences");
+  if (b->tokens > INT32_MAX / 2 || b->table_stride > INT32_MAX || b->max_kv > INT32_MAX / 2)
+    fail(RAI_E_SHAPE, "dimensions overflow");
+  const size_t most = std::min<size_t>(b->max_kv, b->table_stride * p->page_size);
+  *v = BatchView{b->tables, b->table_stride, b->q_start, b->kv_len, (int)b->seqs, (int)b->tokens,
+                 (int)std::min(b->max_q, b->tokens), (int)most};
+  return true;
+}
+
+void check_rows(const void *p, size_t stride, size_t heads, size_t hd, const char *what) {
+  if (!p) fail(RAI_E_ARG, "null argument");
+  if (stride < heads * hd) fail(RAI_E_SHAPE, std::string(what) + " rows overlap: the stride is shorter than a row");
+}
+
+template <class T>
+LayerView<T> layer_view(const rai_pages *p, size_t layer) {
+  const size_t n = layer * p->pages * p->kv_heads * p->page_size * p->head_dim;
+  return {static_cast<T *>(p->k) + n, static_cast<T *>(p->v) + n, (int)p->pages, page_shift(p->page_size),
+          (int)p->kv_heads, (int)p->head_dim};
+}
+
+PoolBytes pool_bytes(const rai_pages *p) {
+  const size_t page = p->kv_heads * p->page_size * p->head_dim * type_bytes(p->type) / 16;
+  return {static_cast<uint4 *>(p->k), static_cast<uint4 *>(p->v), p->pages * page, page, (int)p->layers, (int)p->pages};
+}
+
+// f(LayerView of the pool's type).
+template <class F>
+void with_layer(const rai_pages *p, size_t layer, F f) {
+  if (p->type == RAI_CACHE_F32)
+    f(layer_view<float>(p, layer));
+  else if (p->type == RAI_CACHE_F16)
+    f(layer_view<_Float16>(p, layer));
+  else
+    f(layer_view<Bf16>(p, layer));
+}
+
+void check_heads(size_t heads, const rai_pages *p) {
+  if (heads == 0 || heads % p->kv_heads || heads > 65535)
+    fail(RAI_E_SHAPE, "heads must be a positive multiple of kv_heads");
+}
+
+void check_options(const rai_attention_options *o) {
+  if (!o) fail(RAI_E_ARG, "null argument");
+  if (!std::isfinite(o->scale)) fail(RAI_E_ARG, "scale must be finite");
+  if (!std::isfinite(o->softcap) || o->softcap < 0.0f) fail(RAI_E_ARG, "softcap must be finite and not negative");
+}
+
+int window_of(const rai_attention_options *o) { return (int)std::min<size_t>(o->window, INT32_MAX / 2); }
+
+}  // namespace
+
+}  // namespace rai
+
+extern "C" {
+
+int rai_rope_frequencies(int scaling, double theta, size_t rot, double factor, double trained, double low, double high,
+                         double *inv, float *gain) {
+  RAI_API_BODY({
+    if (!inv || !gain) rai::fail(RAI_E_ARG, "null argument");
+    if (rot == 0 || rot % 2) rai::fail(RAI_E_SHAPE, "rot_dim must be positive and even");
+    if (!std::isfinite(theta) || theta <= 0.0) rai::fail(RAI_E_ARG, "theta must be finite and positive");
+    if (scaling < RAI_ROPE_NONE || scaling > RAI_ROPE_YARN) rai::fail(RAI_E_ARG, "unknown rope scaling");
+    if (scaling != RAI_ROPE_NONE && !(std::isfinite(factor) && factor >= 1.0))
+      rai::fail(RAI_E_ARG, "factor must be finite and at least 1");
+    if (scaling >= RAI_ROPE_LLAMA3 && !(std::isfinite(trained) && trained > 0.0))
+      rai::fail(RAI_E_ARG, "trained_context must be finite and positive");
+    if (scaling == RAI_ROPE_LLAMA3 && !(std::isfinite(high) && low > 0.0 && low < high))
+      rai::fail(RAI_E_ARG, "0 < low_freq < high_freq must hold");
+    if (scaling == RAI_ROPE_YARN && theta == 1.0) rai::fail(RAI_E_ARG, "theta 1 has no wavelengths to blend by");
+    const double two_pi = 6.283185307179586;
+    double lo = 0.0, hi = 1.0;  // YaRN: the pairs (as indexes) that turn 32 times and once in the trained context
+    if (scaling == RAI_ROPE_YARN) {
+      const auto pair_turning = [&](double n) { return rot * std::log(trained / (n * two_pi)) / (2.0 * std::log(theta)); };
+      lo = std::max(std::floor(pair_turning(32.0)), 0.0);
+      hi = std::min(std::ceil(pair_turning(1.0)), (double)rot - 1.0);
+    }
+    for (size_t i = 0; i < rot / 2; ++i) {
+      const double f = std::pow(theta, -2.0 * (double)i / (double)rot);
+      double keep = 1.0;  // share of the unscaled frequency
+      if (scaling == RAI_ROPE_LINEAR) keep = 0.0;
+      if (scaling == RAI_ROPE_LLAMA3) keep = (trained * f / two_pi - low) / (high - low);
+      if (scaling == RAI_ROPE_YARN) keep = 1.0 - ((double)i - lo) / std::max(hi - lo, 0.001);
+      keep = std::min(std::max(keep, 0.0), 1.0);
+      inv[i] = scaling == RAI_ROPE_NONE ? f : f * (keep + (1.0 - keep) / factor);
+    }
+    *gain = scaling == RAI_ROPE_YARN ? (float)(0.1 * std::log(factor) + 1.0) : 1.0f;
+  });
+}
+
+int rai_paged_store_dev(const rai_pages *pages, size_t layer, const rai_page_batch *batch, const rai_rope *rope,
+                        float *q_out, size_t q_out_stride, const float *q, size_t q_stride, size_t heads,
+                        const float *k, size_t k_stride, const float *v, size_t v_stride, void *stream) {
+  RAI_API_BODY({
+    rai::check_pages(pages);
+    if (layer >= pages->layers) rai::fail(RAI_E_RANGE, "layer is out of range");
+    rai::BatchView b;
+    const bool work = rai::check_batch(batch, pages, &b);
+    rai::RopeView r{nullptr, 0, false, 1.0f};
+    if (rope) {
+      if (!rope->inv_freq) rai::fail(RAI_E_ARG, "null argument");
+      if (rope->rot_dim == 0 || rope->rot_dim % 2 || rope->rot_dim > pages->head_dim)
+        rai::fail(RAI_E_SHAPE, "rot_dim must be positive, even and at most head_dim");
+      if (!std::isfinite(rope->gain)) rai::fail(RAI_E_ARG, "gain must be finite");
+      r = rai::RopeView{rope->inv_freq, (int)rope->rot_dim, rope->interleaved != 0, rope->gain};
+    }
+    if (heads > 65535) rai::fail(RAI_E_SHAPE, "dimensions overflow");
+    if (!work) return RAI_OK;
+    if (heads) {
+      rai::check_rows(q, q_stride, heads, pages->head_dim, "q");
+      rai::check_rows(q_out, q_out_stride, heads, pages->head_dim, "q_out");
+      if (q == q_out && q_stride != q_out_stride) rai::fail(RAI_E_SHAPE, "q rotated in place needs one stride");
+    }
+    rai::check_rows(k, k_stride, pages->kv_heads, pages->head_dim, "k");
+    rai::check_rows(v, v_stride, pages->kv_heads, pages->head_dim, "v");
+    const rai::StoreArgs a{q_out, q, k, v, q_out_stride, q_stride, k_stride, v_stride, (int)heads, r};
+    rai::with_layer(pages, layer, [&](auto kv) { rai::launch_store(a, kv, b, (hipStream_t)stream); });
+    RAI_HIP_CHECK(hipGetLastError());
+  });
+}
+
+int rai_paged_attention_workspace(size_t heads, const rai_pages *pages, const rai_page_batch *batch,
+                                  const rai_attention_options *options, size_t *bytes) {
+  RAI_API_BODY({
+    if (!bytes) rai::fail(RAI_E_ARG, "null argument");
+    rai::check_pages(pages);
+    rai::check_heads(heads, pages);
+    rai::check_options(options);
+    rai::BatchView b;
+    *bytes = rai::check_batch(batch, pages, &b)
+                 ? rai::paged_attention_work((int)pages->kv_heads, (int)heads, (int)pages->head_dim, b,
+                                             rai::window_of(options))
+                 : 0;
+  });
+}
+
+int rai_paged_attention_dev(float *out, size_t out_stride, const float *q, size_t q_stride, size_t heads,
+                            const rai_pages *pages, size_t layer, const rai_page_batch *batch,
+                            const rai_attention_options *options, void *work, size_t work_bytes, void *stream) {
+  RAI_API_BODY({
+    rai::check_pages(pages);
+    if (layer >= pages->layers) rai::fail(RAI_E_RANGE, "layer is out of range");
+    rai::check_heads(heads, pages);
+    rai::check_options(options);
+    rai::BatchView b;
+    if (!rai::check_batch(batch, pages, &b)) return RAI_OK;
+    rai::check_rows(q, q_stride, heads, pages->head_dim, "q");
+    rai::check_rows(out, out_stride, heads, pages->head_dim, "out");
+    if (!work && work_bytes) rai::fail(RAI_E_ARG, "null argument");
+    if ((uintptr_t)work % 16) rai::fail(RAI_E_ARG, "work must be 16-byte aligned");
+    const rai::AttnArgs a{q, out, q_stride, out_stride, (int)heads, options->scale, options->softcap,
+                          rai::window_of(options), options->slopes};
+    rai::with_layer(pages, layer,
+                    [&](auto kv) { rai::launch_paged_attention(a, kv, b, work, work_bytes, (hipStream_t)stream); });
+    RAI_HIP_CHECK(hipGetLastError());
+  });
+}
+
+int rai_paged_fork_dev(const rai_pages *pages, const int32_t *tables, size_t table_stride, const int32_t *lengths,
+                       size_t seqs, const int32_t *parent, const int32_t *fresh, size_t n, int32_t *tables_out,
+                       int32_t *lengths_out, int32_t *used, void *stream) {
+  RAI_API_BODY({
+    rai::check_pages(pages);
+    if (n == 0) return RAI_OK;
+    if (!tables || !lengths || !parent || !fresh || !tables_out || !lengths_out || !used)
+      rai::fail(RAI_E_ARG, "null argument");
+    if (seqs == 0 || table_stride == 0) rai::fail(RAI_E_SHAPE, "the tables must not be empty");
+    if (n > 65535 || seqs > 65535) rai::fail(RAI_E_SHAPE, "at most 65535 sequences");
+    if (table_stride > INT32_MAX) rai::fail(RAI_E_SHAPE, "dimensions overflow");
+    if (tables_out < tables + seqs * table_stride && tables < tables_out + n * table_stride)
+      rai::fail(RAI_E_ARG, "tables_out overlaps tables");
+    if (lengths_out < lengths + seqs && lengths < lengths_out + n) rai::fail(RAI_E_ARG, "lengths_out overlaps lengths");
+    const rai::PoolBytes p = rai::pool_bytes(pages);
+    rai::k_fork<<<dim3(p.layers, n), 256, 0, (hipStream_t)stream>>>(p, tables, table_stride, lengths, (int)seqs, parent,
+                                                                    fresh, (int)n, tables_out, lengths_out, used,
+                                                                    rai::page_shift(pages->page_size));
+    RAI_HIP_CHECK(hipGetLastError());
+  });
+}
+
+int rai_paged_move_dev(const rai_pages *pages, const int32_t *src, const int32_t *dst, size_t n, int32_t *tables,
+                       size_t entries, void *stream) {
+  RAI_API_BODY({
+    rai::check_pages(pages);
+    if (n == 0) return RAI_OK;
+    if (!src || !dst || (!tables && entries)) rai::fail(RAI_E_ARG, "null argument");
+    if (n > 65535) rai::fail(RAI_E_SHAPE, "at most 65535 pages in one call");
+    const rai::PoolBytes p = rai::pool_bytes(pages);
+    hipStream_t s = (hipStream_t)stream;
+    rai::k_move<<<dim3(p.layers, n), 256, 0, s>>>(p, src, dst, (int)n);
+    if (entries)
+      rai::k_rename<<<(int)std::min<size_t>(1024, (entries + 255) / 256), 256, 0, s>>>(src, dst, (int)n, p.pages,
+                                                                                      tables, entries);
+    RAI_HIP_CHECK(hipGetLastError());
+  });
+}
+
+}  // extern "C"
