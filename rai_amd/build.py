@@ -30,7 +30,7 @@ SOURCES = ["kernels.hip", "fused.hip", "attn_mm.hip", "gemv.hip", "gemv_stream.h
 # compiler routes them through AGPRs and one copy per value).
 EXTRA = {"gemv.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"], "gemm_mm.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"],
          "gemv_stream.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"],
-         "attn_mm.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"]}
+         "attn_mm.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"], "paged_attn.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"]}
 
 
 def _compile(src: str) -> str:

@@ -247,6 +247,11 @@ void check_heads(size_t heads, const rai_pages *p) {
     fail(RAI_E_SHAPE, "heads must be a positive multiple of kv_heads");
 }
 
+// Rows of a batch, head by head: the launches' bound.
+void check_rows_heads(const BatchView &b, size_t heads) {
+  if ((size_t)b.tokens * heads >= size_t(1) << 24) fail(RAI_E_SHAPE, "at most 2^24 - 1 rows x heads in one call");
+}
+
 void check_options(const rai_attention_options *o) {
   if (!o) fail(RAI_E_ARG, "null argument");
   if (!std::isfinite(o->scale)) fail(RAI_E_ARG, "scale must be finite");
@@ -334,10 +339,11 @@ int rai_paged_attention_workspace(size_t heads, const rai_pages *pages, const ra
     rai::check_heads(heads, pages);
     rai::check_options(options);
     rai::BatchView b;
-    *bytes = rai::check_batch(batch, pages, &b)
-                 ? rai::paged_attention_work((int)pages->kv_heads, (int)heads, (int)pages->head_dim, b,
-                                             rai::window_of(options))
-                 : 0;
+    *bytes = 0;
+    if (!rai::check_batch(batch, pages, &b)) return RAI_OK;
+    rai::check_rows_heads(b, heads);
+    *bytes = rai::paged_attention_work((int)pages->kv_heads, (int)heads, (int)pages->head_dim, b,
+                                       rai::window_of(options));
   });
 }
 
@@ -351,6 +357,7 @@ int rai_paged_attention_dev(float *out, size_t out_stride, const float *q, size_
     rai::check_options(options);
     rai::BatchView b;
     if (!rai::check_batch(batch, pages, &b)) return RAI_OK;
+    rai::check_rows_heads(b, heads);
     rai::check_rows(q, q_stride, heads, pages->head_dim, "q");
     rai::check_rows(out, out_stride, heads, pages->head_dim, "out");
     if (!work && work_bytes) rai::fail(RAI_E_ARG, "null argument");

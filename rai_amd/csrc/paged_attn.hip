@@ -3,7 +3,27 @@
 //   out = sum_j p_j v_j / sum_j p_j,  p_j = exp(s_j - max s),  s_j = cap(q . k_j scale) - slope (pos - j)
 //
 // over the positions j that a row sees, in one pass with the running maximum and
-// sum of the softmax, all in f32.
+// sum of the softmax.  The rows of one kv head (new tokens x the query heads on
+// it) share its keys and values: S^T = K Q^T and O^T = V^T P^T are tiles of the
+// 16-bit matrix instructions, with f32 sums.
+//
+// f32 accuracy from 16-bit operands.  An f32 value is the exact sum of three bf16
+// ones (8 + 8 + 8 bits, each cut off), so a product with a bf16 value is three
+// exact products, and one of two f32 values the six of nine whose weight reaches
+// 2^-24.  Against f16 values two f16 parts do (11 + 11 bits and the sign of the
+// second), the queries of a row scaled by a power of two so that the range of f16
+// cannot cut them, the probabilities by 2^14.  The f32 matrix instructions run at
+// a sixteenth of the 16-bit rate: three or six products are the faster way.
+//
+// Layout.  The instruction leaves row 4 g + i (16 x 16) or 8 b + 4 h + c (32 x 32)
+// of S^T in lane group g or h; the keys are dealt to the rows so that a lane ends
+// up with eight keys in a row for one query, which is what the second product
+// takes as its operand: the probabilities never leave their lane.
+//
+// Results that are not finite (a NaN or an infinity in what the row sees, or in
+// what a neighbour sees: 0 x inf in the shared products) are computed again row by
+// row, from the keys that the row sees alone.
+#include "kernels.h"
 #include "paged.h"
 
 #include <algorithm>
@@ -14,6 +34,13 @@ namespace rai {
 namespace {
 
 constexpr float kLog2e = 1.4426950408889634f;
+
+typedef float f4 __attribute__((ext_vector_type(4)));
+typedef float f16v __attribute__((ext_vector_type(16)));
+typedef uint32_t u4 __attribute__((ext_vector_type(4)));
+typedef _Float16 h8 __attribute__((ext_vector_type(8)));
+typedef _Float16 h2 __attribute__((ext_vector_type(2)));
+typedef __bf16 b8 __attribute__((ext_vector_type(8)));
 
 __device__ __forceinline__ float wave_max(float x) {
 #pragma unroll
@@ -26,15 +53,76 @@ __device__ __forceinline__ float wave_sum(float x) {
   return x;
 }
 
+// tanh: odd polynomial near zero (1 - 2 / (e^2x + 1) cancels there), error under
+// 2^-22 relative.
+__device__ __forceinline__ float cap_tanh(float x) {
+  const float a = fabsf(x);
+  const float e = __builtin_amdgcn_exp2f(2.0f * kLog2e * a);
+  const float far = 1.0f - 2.0f * __builtin_amdgcn_rcpf(e + 1.0f);
+  const float y = a * a;
+  const float near =
+      a + a * y * (-0.33333333f + y * (0.13333333f + y * (-0.053968254f + y * (0.021869488f - y * 0.0088632355f))));
+  return copysignf(a < 0.4f ? near : far, x);
+}
+
+// A score in the log2 domain: x = q . k * scale.
+struct Score {
+  float softcap, inv_cap, slope;
+  bool plain;
+  __device__ __forceinline__ float operator()(float x, int away) const {
+    if (plain) return x * kLog2e;
+    if (softcap > 0.0f) x = softcap * cap_tanh(x * inv_cap);
+    return (x - slope * (float)away) * kLog2e;
+  }
+};
+__device__ __forceinline__ Score score_of(const AttnArgs &a, int head) {
+  return {a.softcap, a.softcap > 0.0f ? 1.0f / a.softcap : 0.0f, a.slopes ? a.slopes[head] : 0.0f,
+          a.softcap == 0.0f && !a.slopes};
+}
+
+// ------------------------------------------------------------ rows and splits --
+
+// Rows of a sequence on one kv head: r = token * per + query head of the group.
+// Tile t holds rows t * R .. of them and reads positions lo .. hi - 1; a split is
+// `len` of those, from `lo` rounded down to a whole stage.
+struct Tile {
+  int lo, hi;  // lo: a multiple of 64
+};
+__device__ __forceinline__ Tile tile_of(const SeqSpan &sp, int t, int R, int per, int window) {
+  const int base = sp.n - sp.nq, first = t * R / per, last = min(sp.nq - 1, (t * R + R - 1) / per);
+  return {first_seen(base + first, window) & ~63, max(base + last + 1, 0)};
+}
+__device__ __forceinline__ int splits_of(const Tile &t, int len) { return t.hi > t.lo ? (t.hi - t.lo + len - 1) / len : 1; }
+
+constexpr int kFewRows = 16;    // a tile of k_few
+constexpr int kManyRows = 128;  // a tile of k_many
+
+// Sequences of at most kFewRows rows a kv head go to k_few, others to k_many.
+__device__ __forceinline__ bool few_rows(int nq, int per) { return nq * per <= kFewRows; }
+
+// How the key axis is split, and where the parts of a row's softmax lie:
+// [split][token row][head] x (hd values), and maximum and sum behind them.
+struct Splits {
+  int few_len, many_len, most;
+  float *o;
+  float2 *ml;
+};
+
+__device__ __forceinline__ size_t part_at(const AttnArgs &a, const BatchView &b, int split, int row, int head) {
+  return ((size_t)split * b.tokens + row) * a.heads + head;
+}
+
+// -------------------------------------------------------------------- one row --
+
 // One row of one head by one wave: positions lo .. hi - 1 of the sequence whose
 // table row is `table`, lane t holding key base + t and dimensions t, t + 64, ...
 // of the output.  Keys that are not there or masked are not read into the sums at
-// all, whatever they hold.
+// all, whatever they hold.  m is in the log2 domain.
 template <class T>
 __device__ void wave_row(const AttnArgs &a, const LayerView<T> &kv, const int *table, int head, const float *q, int pos,
                          int lo, int hi, float &m, float &l, float (&o)[4]) {
   const int lane = threadIdx.x & 63, hd = kv.hd, kvh = head / (a.heads / kv.nkv), mask = (1 << kv.shift) - 1;
-  const float slope = a.slopes ? a.slopes[head] : 0.0f;
+  const Score score = score_of(a, head);
   m = -INFINITY;
   l = 0.0f;
 #pragma unroll
@@ -47,14 +135,12 @@ __device__ void wave_row(const AttnArgs &a, const LayerView<T> &kv, const int *t
       const T *k = kv.k + key_at(page, kvh, j & mask, kv.nkv, hd, kv.shift);
       float d = 0.0f;
       for (int e = 0; e < hd; ++e) d = fmaf(q[e], to_f32(k[e]), d);
-      s = d * a.scale;
-      if (a.softcap > 0.0f) s = a.softcap * tanhf(s / a.softcap);
-      s -= slope * (float)(pos - j);
+      s = score(d * a.scale, pos - j);
     }
     float mn = fmaxf(m, wave_max(s));
     if (__any(s != s)) mn = NAN;
     if (mn == -INFINITY) continue;
-    const float scale = exp2f((m - mn) * kLog2e), p = exp2f((s - mn) * kLog2e);
+    const float scale = exp2f(m - mn), p = exp2f(s - mn);
     l = l * scale + wave_sum(p);
 #pragma unroll
     for (int i = 0; i < 4; ++i) o[i] *= scale;
@@ -71,32 +157,737 @@ __device__ void wave_row(const AttnArgs &a, const LayerView<T> &kv, const int *t
   }
 }
 
-// A wave per (row, head).
+// A row's result again, from its own keys of positions lo .. hi - 1 (of the split).
 template <class T>
-__global__ __launch_bounds__(256) void k_rows(AttnArgs a, LayerView<T> kv, BatchView b) {
-  const SeqSpan sp = seq_span(b, blockIdx.y);
-  const int unit = blockIdx.x * 4 + (threadIdx.x >> 6), j = unit / a.heads, head = unit % a.heads, lane = threadIdx.x & 63;
-  if (j >= sp.nq) return;
-  const int pos = sp.n - sp.nq + j;
+__device__ __noinline__ void redo_row(const AttnArgs &a, const LayerView<T> &kv, const BatchView &b, const Splits &sl,
+                                      const int *table, int row, int head, int pos, int lo, int hi, int split,
+                                      int splits) {
+  const int lane = threadIdx.x & 63;
   float m, l, o[4];
-  wave_row(a, kv, b.tables + (size_t)blockIdx.y * b.stride, head,
-           a.q + (size_t)(sp.q0 + j) * a.q_stride + (size_t)head * kv.hd, pos, first_seen(pos, a.window), pos + 1, m, l,
-           o);
-  float *out = a.out + (size_t)(sp.q0 + j) * a.out_stride + (size_t)head * kv.hd;
+  wave_row(a, kv, table, head, a.q + (size_t)row * a.q_stride + (size_t)head * kv.hd, pos,
+           max(lo, first_seen(pos, a.window)), min(hi, pos + 1), m, l, o);
+  float *out = a.out + (size_t)row * a.out_stride + (size_t)head * kv.hd;
+  if (splits > 1) {
+    const size_t at = part_at(a, b, split, row, head);
+    out = sl.o + at * kv.hd;
+    if (lane == 0) sl.ml[at] = make_float2(m, l);
+    l = 1.0f;
+  }
 #pragma unroll
   for (int i = 0; i < 4; ++i)
     if (lane + 64 * i < kv.hd) out[lane + 64 * i] = l == 0.0f ? 0.0f : o[i] / l;
 }
 
+// ------------------------------------------------------------- 16-bit operands --
+
+// Eight values of the cache as a matrix operand, in KP parts; P parts of an f32
+// operand against them; the products that count, largest last.
+template <class T>
+struct Form;
+
+__device__ __forceinline__ u4 cut3(const float (&x)[8], u4 &mid, u4 &low) {
+  u4 h;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const uint32_t a = __float_as_uint(x[2 * i]), b = __float_as_uint(x[2 * i + 1]);
+    h[i] = __builtin_amdgcn_perm(b, a, 0x07060302);
+    const float ra = x[2 * i] - __uint_as_float(a & 0xffff0000u), rb = x[2 * i + 1] - __uint_as_float(b & 0xffff0000u);
+    const uint32_t c = __float_as_uint(ra), d = __float_as_uint(rb);
+    mid[i] = __builtin_amdgcn_perm(d, c, 0x07060302);
+    const float la = ra - __uint_as_float(c & 0xffff0000u), lb = rb - __uint_as_float(d & 0xffff0000u);
+    low[i] = __builtin_amdgcn_perm(__float_as_uint(lb), __float_as_uint(la), 0x07060302);
+  }
+  return h;
+}
+
+struct Bf16Form {
+  static constexpr int P = 3;
+  static constexpr float kLift = 0.0f;
+  static __device__ __forceinline__ f4 mma16(u4 x, u4 y, f4 c) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(b8, x), __builtin_bit_cast(b8, y), c, 0, 0, 0);
+  }
+  static __device__ __forceinline__ f16v mma32(u4 x, u4 y, f16v c) {
+    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(b8, x), __builtin_bit_cast(b8, y), c, 0, 0, 0);
+  }
+  static __device__ __forceinline__ void parts(const float (&x)[8], u4 (&p)[3]) { p[0] = cut3(x, p[1], p[2]); }
+  static __device__ __forceinline__ int row_exponent(float) { return 0; }
+};
+template <>
+struct Form<float> : Bf16Form {
+  static constexpr int KP = 3;
+};
+template <>
+struct Form<Bf16> : Bf16Form {
+  static constexpr int KP = 1;
+};
+template <>
+struct Form<_Float16> {
+  static constexpr int P = 2, KP = 1;
+  static constexpr float kLift = 14.0f;  // probabilities times 2^14: f16's subnormals start 2^-28 below the largest
+  static __device__ __forceinline__ f4 mma16(u4 x, u4 y, f4 c) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(h8, x), __builtin_bit_cast(h8, y), c, 0, 0, 0);
+  }
+  static __device__ __forceinline__ f16v mma32(u4 x, u4 y, f16v c) {
+    return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(h8, x), __builtin_bit_cast(h8, y), c, 0, 0, 0);
+  }
+  static __device__ __forceinline__ void parts(const float (&x)[8], u4 (&p)[2]) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const h2 h = {(_Float16)x[2 * i], (_Float16)x[2 * i + 1]};
+      const h2 l = {(_Float16)(x[2 * i] - (float)h[0]), (_Float16)(x[2 * i + 1] - (float)h[1])};
+      p[0][i] = __builtin_bit_cast(uint32_t, h);
+      p[1][i] = __builtin_bit_cast(uint32_t, l);
+    }
+  }
+  // The power of two that brings a row's largest value to 2^14..2^15.
+  static __device__ __forceinline__ int row_exponent(float most) {
+    return most > 0.0f && most < INFINITY ? 14 - ilogbf(most) : 0;
+  }
+};
+
+// c += the product of a cache operand x (KP parts) and an f32 operand y (P parts).
+template <class F, class C, int KP, int P, class M>
+__device__ __forceinline__ C products(const u4 (&x)[KP], const u4 (&y)[P], C c, M mma) {
+#pragma unroll
+  for (int w = KP + P - 2 < P - 1 ? KP + P - 2 : P - 1; w >= 0; --w)  // parts i + j = w, smallest first
+#pragma unroll
+    for (int i = 0; i < KP; ++i)
+      if (w - i >= 0 && w - i < P) c = mma(x[i], y[w - i], c);
+  return c;
+}
+
+// Eight cache values in flight, and as the parts of an operand.
+template <class T>
+struct Raw {
+  u4 v[sizeof(T) / 2];
+  __device__ __forceinline__ void load(const T *p) {
+#pragma unroll
+    for (int i = 0; i < (int)sizeof(T) / 2; ++i) v[i] = reinterpret_cast<const u4 *>(p)[i];
+  }
+  __device__ __forceinline__ void zero() {
+#pragma unroll
+    for (int i = 0; i < (int)sizeof(T) / 2; ++i) v[i] = u4{0, 0, 0, 0};
+  }
+  // Keeps elements from .. to - 1 of the eight.
+  __device__ __forceinline__ void keep(int from, int to) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      const bool in = e >= from && e < to;
+      if constexpr (sizeof(T) == 4)
+        v[e / 4][e % 4] = in ? v[e / 4][e % 4] : 0u;
+      else
+        v[0][e / 2] = in ? v[0][e / 2] : v[0][e / 2] & (e % 2 ? 0x0000ffffu : 0xffff0000u);
+    }
+  }
+  __device__ __forceinline__ void parts(u4 (&x)[Form<T>::KP]) const {
+    if constexpr (sizeof(T) == 4) {
+      float f[8];
+#pragma unroll
+      for (int e = 0; e < 8; ++e) f[e] = __uint_as_float(v[e / 4][e % 4]);
+      x[0] = cut3(f, x[1], x[2]);
+    } else {
+      x[0] = v[0];
+    }
+  }
+};
+
+// Query values e .. e + 7 of a row (zero from hd on); `vec`: 16-byte loads fit.
+__device__ __forceinline__ void query8(const float *q, int e, int hd, bool vec, float (&x)[8]) {
+  if (e >= hd) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) x[i] = 0.0f;
+  } else if (vec) {
+    const f4 a = *reinterpret_cast<const f4 *>(q + e), b = *reinterpret_cast<const f4 *>(q + e + 4);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) x[i] = a[i], x[4 + i] = b[i];
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) x[i] = q[e + i];
+  }
+}
+
+__device__ __forceinline__ bool finite4(f4 x) {
+  return fabsf(x[0]) < INFINITY && fabsf(x[1]) < INFINITY && fabsf(x[2]) < INFINITY && fabsf(x[3]) < INFINITY;
+}
+
+// -------------------------------------------------------------------- few rows --
+
+// At most 16 rows a kv head: one token of a sequence, or a verify batch.  Block
+// (split, kv head, sequence); the keys go to the waves 32 at a time, straight from
+// the pages into the operands (each is read once, so there is nothing to stage),
+// and the waves' softmaxes are joined in LDS.
+template <class T, int HC>  // HC: head size in steps of 32, rounded up
+__global__ __launch_bounds__(256) void k_few(AttnArgs a, LayerView<T> kv, BatchView b, Splits sl, bool vec) {
+  using F = Form<T>;
+  constexpr int KP = F::KP, P = F::P, D = 2 * HC;
+  __shared__ float ml[2][4][16];
+  __shared__ f4 part[2][D][64];
+  __shared__ uint32_t bad_rows;
+  const int seq = blockIdx.z, kvh = blockIdx.y, split = blockIdx.x, per = a.heads / kv.nkv, hd = kv.hd;
+  const SeqSpan sp = seq_span(b, seq);
+  const int rows = sp.nq * per;
+  if (rows == 0 || !few_rows(sp.nq, per)) return;
+  const Tile tile = tile_of(sp, 0, kFewRows, per, a.window);
+  const int splits = splits_of(tile, sl.few_len);
+  if (split >= splits) return;
+  const int lo = tile.lo + split * sl.few_len, hi = min(tile.hi, lo + sl.few_len);
+  const int seen = first_seen(sp.n - sp.nq, a.window);  // no row sees less
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, col = lane & 15, g = lane >> 4;
+  const int *table = b.tables + (size_t)seq * b.stride;
+  const int mask = (1 << kv.shift) - 1;
+  // The row of this lane's column.
+  const int r = min(col, rows - 1), tok = r / per, head = kvh * per + r % per, pos = sp.n - sp.nq + tok;
+  const int first = first_seen(pos, a.window);
+  const Score score = score_of(a, head);
+  u4 q[HC][P];
+  float back;
+  {
+    const float *x = a.q + (size_t)(sp.q0 + tok) * a.q_stride + (size_t)head * hd;
+    float v[HC][8], most = 0.0f;
+#pragma unroll
+    for (int c = 0; c < HC; ++c) {
+      query8(x, 32 * c + 8 * g, hd, vec, v[c]);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) most = fmaxf(most, fabsf(v[c][i]));
+    }
+    most = fmaxf(most, __shfl_xor(most, 16));
+    most = fmaxf(most, __shfl_xor(most, 32));
+    const int up = F::row_exponent(most);
+#pragma unroll
+    for (int c = 0; c < HC; ++c) {
+      if (up)
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[c][i] = ldexpf(v[c][i], up);
+      F::parts(v[c], q[c]);
+    }
+    back = ldexpf(a.scale, -up);
+  }
+  f4 o[D];
+#pragma unroll
+  for (int d = 0; d < D; ++d) o[d] = f4{0, 0, 0, 0};
+  float m = -INFINITY, l = 0.0f;
+  for (int base = lo + 32 * wave; base < hi; base += 128) {
+    // Lane's key rows of the two score tiles: base + 8 (col / 4) + 4 t + col % 4;
+    // its keys in S^T and in V^T: base + 8 g ...
+    const int kk = base + 8 * (col >> 2), vk = base + 8 * g;
+    const int kpage = kk < hi ? page_of(table, kk, kv.shift, kv.pages) : -1;
+    const int vpage = vk < hi ? page_of(table, vk, kv.shift, kv.pages) : -1;
+    Raw<T> kr[2][HC], vr[D];
+#pragma unroll
+    for (int t = 0; t < 2; ++t) {
+      const int key = kk + 4 * t + (col & 3);
+      const bool in = kpage >= 0 && key < hi && key >= seen;
+      const T *p = kv.k + key_at(max(kpage, 0), kvh, key & mask, kv.nkv, hd, kv.shift) + 8 * g;
+#pragma unroll
+      for (int c = 0; c < HC; ++c) {
+        if (in && 32 * c + 8 * g < hd)
+          kr[t][c].load(p + 32 * c);
+        else
+          kr[t][c].zero();
+      }
+    }
+    {
+      const T *p = kv.v + value_at(max(vpage, 0), kvh, vk & mask, kv.nkv, hd, kv.shift) + ((size_t)col << kv.shift);
+#pragma unroll
+      for (int d = 0; d < D; ++d) {
+        if (vpage >= 0 && 16 * d + col < hd)
+          vr[d].load(p + ((size_t)(16 * d) << kv.shift));
+        else
+          vr[d].zero();
+      }
+    }
+    f4 s[2] = {f4{0, 0, 0, 0}, f4{0, 0, 0, 0}};
+#pragma unroll
+    for (int c = 0; c < HC; ++c)
+#pragma unroll
+      for (int t = 0; t < 2; ++t) {
+        u4 x[KP];
+        kr[t][c].parts(x);
+        s[t] = products<F>(x, q[c], s[t], [](u4 x, u4 y, f4 c) { return F::mma16(x, y, c); });
+      }
+    float x[8], top = -INFINITY;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      const int key = vk + e;
+      const bool in = vpage >= 0 && key <= pos && key >= first && key < hi;
+      x[e] = in ? score(s[e / 4][e % 4] * back, pos - key) : -INFINITY;
+      top = fmaxf(top, x[e]);
+    }
+    top = fmaxf(top, __shfl_xor(top, 16));
+    top = fmaxf(top, __shfl_xor(top, 32));
+    const float mn = fmaxf(m, top), ref = (mn == -INFINITY ? 0.0f : mn) - F::kLift;
+    const float alpha = m == mn ? 1.0f : __builtin_amdgcn_exp2f(m - mn);
+    m = mn;
+    float sum = 0.0f;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      x[e] = __builtin_amdgcn_exp2f(x[e] - ref);
+      sum += x[e];
+    }
+    l = l * alpha + sum;
+    if (__any(alpha != 1.0f))
+#pragma unroll
+      for (int d = 0; d < D; ++d) o[d] *= alpha;
+    u4 p[P];
+    F::parts(x, p);
+    // Slots that hold no key of these rows: whatever lies there stays out.
+    const bool edge = base < seen || base + 32 > hi;
+#pragma unroll
+    for (int d = 0; d < D; ++d) {
+      if (edge) vr[d].keep(seen - vk, hi - vk);
+      u4 y[KP];
+      vr[d].parts(y);
+      o[d] = products<F>(y, p, o[d], [](u4 x, u4 y, f4 c) { return F::mma16(x, y, c); });
+    }
+  }
+  // The four waves' softmaxes, then the four lane groups' shares of the sum.
+  l += __shfl_xor(l, 16);
+  l += __shfl_xor(l, 32);
+  if (g == 0) ml[0][wave][col] = m, ml[1][wave][col] = l;
+  __syncthreads();
+  float top = ml[0][0][col];
+#pragma unroll
+  for (int w = 1; w < 4; ++w) top = fmaxf(top, ml[0][w][col]);
+  float sum = 0.0f;
+#pragma unroll
+  for (int w = 0; w < 4; ++w) {
+    const float mw = ml[0][w][col];
+    sum += ml[1][w][col] * (mw == top ? 1.0f : __builtin_amdgcn_exp2f(mw - top));
+  }
+  const float mine = m == top ? 1.0f : __builtin_amdgcn_exp2f(m - top);
+#pragma unroll
+  for (int d = 0; d < D; ++d) o[d] *= mine;
+#pragma unroll
+  for (int from = 2; from; from >>= 1) {
+    if (wave >= from && wave < 2 * from)
+#pragma unroll
+      for (int d = 0; d < D; ++d) part[wave - from][d][lane] = o[d];
+    __syncthreads();
+    if (wave < from)
+#pragma unroll
+      for (int d = 0; d < D; ++d) o[d] += part[wave][d][lane];
+    __syncthreads();
+  }
+  if (wave == 0) {
+    bool bad = !(fabsf(sum) < INFINITY);
+#pragma unroll
+    for (int d = 0; d < D; ++d) bad = bad || !finite4(o[d]);
+    const uint64_t all = __ballot(bad);
+    if (lane == 0) bad_rows = (uint32_t)(all | all >> 16 | all >> 32 | all >> 48) & 0xffffu;
+    if (col < rows) {
+      const size_t at = part_at(a, b, split, sp.q0 + tok, head);
+      float *out = a.out + (size_t)(sp.q0 + tok) * a.out_stride + (size_t)head * hd;
+      float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+      bool wide = vec;
+      if (splits > 1) {
+        out = sl.o + at * hd;
+        if (g == 0) sl.ml[at] = make_float2(top - F::kLift, sum);
+        inv = 1.0f;
+        wide = true;
+      }
+#pragma unroll
+      for (int d = 0; d < D; ++d) {
+        const int e = 16 * d + 4 * g;
+        if (e >= hd) continue;
+        const f4 y = o[d] * inv;
+        if (wide)
+          *reinterpret_cast<f4 *>(out + e) = y;
+        else
+          for (int i = 0; i < 4; ++i) out[e + i] = y[i];
+      }
+    }
+  }
+  __syncthreads();
+  if (bad_rows == 0) return;
+  for (int i = wave; i < rows; i += 4)
+    if (bad_rows >> i & 1)
+      redo_row(a, kv, b, sl, table, sp.q0 + i / per, kvh * per + i % per, sp.n - sp.nq + i / per, lo, hi, split, splits);
+}
+
+// ------------------------------------------------------------------- many rows --
+
+// Chunks of a prompt.  Block (row tile x kv head, split, sequence): each of four
+// waves has 32 rows, and a stage of keys and values passes through LDS for all of
+// them, lying there operand by operand (lane after lane, so that reads are linear
+// and f32 values are cut into their parts once for the block).  The next stage's
+// values come from the pages while a stage is worked on.
+template <class T>
+constexpr int kStage = sizeof(T) == 4 ? 32 : 64;
+
+template <class T, int HC>
+constexpr size_t many_lds() {
+  return (size_t)2 * kStage<T> * HC * 32 * 2 * Form<T>::KP;
+}
+
+// Row of a 32 x 32 operand that holds key k of its 32.
+__device__ __forceinline__ int key_row(int k) { return (k & 16) + 2 * (k & 4) + ((k & 8) >> 1) + (k & 3); }
+
+template <class T, int HC>
+__global__ __launch_bounds__(256) void k_many(AttnArgs a, LayerView<T> kv, BatchView b, Splits sl, bool vec) {
+  using F = Form<T>;
+  constexpr int KP = F::KP, P = F::P, S = kStage<T>, SUB = S / 32, KS = 2 * HC, UNITS = S * HC * 4, U = (UNITS + 255) / 256;
+  extern __shared__ __align__(16) uint8_t lds[];
+  u4 *kl = reinterpret_cast<u4 *>(lds), *vl = kl + SUB * KS * KP * 64;
+  const int seq = blockIdx.z, split = blockIdx.y, per = a.heads / kv.nkv, hd = kv.hd;
+  const SeqSpan sp = seq_span(b, seq);
+  const int rows = sp.nq * per, tiles = (rows + kManyRows - 1) / kManyRows;
+  // Kv heads side by side (an XCD keeps those of its own in L2), the longest rows first.
+  const int kvh = blockIdx.x % kv.nkv, t = tiles - 1 - (int)(blockIdx.x / kv.nkv);
+  if (t < 0 || few_rows(sp.nq, per)) return;
+  const Tile tile = tile_of(sp, t, kManyRows, per, a.window);
+  const int splits = splits_of(tile, sl.many_len);
+  if (split >= splits) return;
+  const int lo = tile.lo + split * sl.many_len, hi = min(tile.hi, lo + sl.many_len);
+  const int base0 = sp.n - sp.nq;
+  const int seen = first_seen(base0 + t * kManyRows / per, a.window);
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, col = lane & 31, h = lane >> 5;
+  const int *table = b.tables + (size_t)seq * b.stride;
+  const int mask = (1 << kv.shift) - 1;
+  const int r0 = t * kManyRows + 32 * wave, r = min(r0 + col, rows - 1), tok = r / per, head = kvh * per + r % per;
+  const int pos = base0 + tok, first = first_seen(pos, a.window);
+  // The wave's rows see nothing before wlo, nothing from whi on; all of them see
+  // everything between alo and ahi.
+  const int tok0 = min(r0, rows - 1) / per, tok1 = min(r0 + 31, rows - 1) / per;
+  const bool idle = r0 >= rows;
+  const int wlo = first_seen(base0 + tok0, a.window), whi = base0 + tok1 + 1;
+  const int alo = first_seen(base0 + tok1, a.window), ahi = base0 + tok0 + 1;
+  const Score score = score_of(a, head);
+  u4 q[KS][P];
+  float back;
+  {
+    const float *x = a.q + (size_t)(sp.q0 + tok) * a.q_stride + (size_t)head * hd;
+    float most = 0.0f;
+    int up = 0;
+    if (F::kLift != 0.0f) {  // f16
+      for (int c = 0; c < KS; ++c) {
+        float v[8];
+        query8(x, 16 * c + 8 * h, hd, vec, v);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) most = fmaxf(most, fabsf(v[i]));
+      }
+      most = fmaxf(most, __shfl_xor(most, 32));
+      up = F::row_exponent(most);
+    }
+#pragma unroll
+    for (int c = 0; c < KS; ++c) {
+      float v[8];
+      query8(x, 16 * c + 8 * h, hd, vec, v);
+      if (F::kLift != 0.0f)
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[i] = ldexpf(v[i], up);
+      F::parts(v, q[c]);
+    }
+    back = ldexpf(a.scale, -up);
+  }
+  f16v o[HC];
+#pragma unroll
+  for (int d = 0; d < HC; ++d)
+#pragma unroll
+    for (int i = 0; i < 16; ++i) o[d][i] = 0.0f;
+  float m = -INFINITY, l = 0.0f;
+
+  // Unit u of a stage's keys: 16 keys x 4 chunks of 8 dimensions per 64 units; of
+  // its values: 16 dimensions x 4 chunks of 8 keys.
+  Raw<T> kr[U], vr[U];
+  auto key_unit = [](int u, int &key, int &chunk) {
+    key = (u & 15) + 16 * ((u >> 6) % (S / 16));
+    chunk = ((u >> 4) & 3) + 4 * ((u >> 6) / (S / 16));
+  };
+  auto value_unit = [](int u, int &d, int &chunk) {
+    d = (u & 15) + 16 * ((u >> 6) % (2 * HC));
+    chunk = ((u >> 4) & 3) + 4 * ((u >> 6) / (2 * HC));
+  };
+  auto load = [&](int base) {
+#pragma unroll
+    for (int i = 0; i < U; ++i) {
+      int key, chunk;
+      key_unit(tid + 256 * i, key, chunk);
+      key += base;
+      const int page = key < hi ? page_of(table, key, kv.shift, kv.pages) : -1;
+      if (page >= 0 && key >= seen && 8 * chunk < hd && (UNITS % 256 == 0 || tid + 256 * i < UNITS))
+        kr[i].load(kv.k + key_at(page, kvh, key & mask, kv.nkv, hd, kv.shift) + 8 * chunk);
+      else
+        kr[i].zero();
+    }
+#pragma unroll
+    for (int i = 0; i < U; ++i) {
+      int d, chunk;
+      value_unit(tid + 256 * i, d, chunk);
+      const int key = base + 8 * chunk;
+      const int page = key < hi ? page_of(table, key, kv.shift, kv.pages) : -1;
+      if (page >= 0 && d < hd && (UNITS % 256 == 0 || tid + 256 * i < UNITS))
+        vr[i].load(kv.v + value_at(page, kvh, key & mask, kv.nkv, hd, kv.shift) + ((size_t)d << kv.shift));
+      else
+        vr[i].zero();
+    }
+  };
+  auto put = [&](int base) {
+    const bool edge = base < seen || base + S > hi;
+#pragma unroll
+    for (int i = 0; i < U; ++i) {
+      int key, chunk;
+      key_unit(tid + 256 * i, key, chunk);
+      if (UNITS % 256 && tid + 256 * i >= UNITS) break;
+      u4 x[KP];
+      kr[i].parts(x);
+      u4 *to = kl + ((key >> 5) * KS + (chunk >> 1)) * KP * 64 + (chunk & 1) * 32 + key_row(key & 31);
+#pragma unroll
+      for (int j = 0; j < KP; ++j) to[j * 64] = x[j];
+    }
+#pragma unroll
+    for (int i = 0; i < U; ++i) {
+      int d, chunk;
+      value_unit(tid + 256 * i, d, chunk);
+      if (UNITS % 256 && tid + 256 * i >= UNITS) break;
+      if (edge) vr[i].keep(seen - base - 8 * chunk, hi - base - 8 * chunk);
+      u4 x[KP];
+      vr[i].parts(x);
+      u4 *to = vl + ((chunk >> 1) * HC + (d >> 5)) * KP * 64 + (chunk & 1) * 32 + (d & 31);
+#pragma unroll
+      for (int j = 0; j < KP; ++j) to[j * 64] = x[j];
+    }
+  };
+
+  load(lo);
+  for (int base = lo; base < hi; base += S) {
+    put(base);
+    __syncthreads();
+    if (base + S < hi) load(base + S);
+#pragma unroll
+    for (int sub = 0; sub < SUB; ++sub) {
+      const int kb = base + 32 * sub;
+      if (idle || kb >= whi || kb + 32 <= wlo) continue;
+      f16v s;
+#pragma unroll
+      for (int i = 0; i < 16; ++i) s[i] = 0.0f;
+#pragma unroll
+      for (int c = 0; c < KS; ++c) {
+        u4 x[KP];
+#pragma unroll
+        for (int j = 0; j < KP; ++j) x[j] = kl[((sub * KS + c) * KP + j) * 64 + lane];
+        s = products<F>(x, q[c], s, [](u4 x, u4 y, f16v c) { return F::mma32(x, y, c); });
+      }
+      // Register 8 u + j of a lane is key kb + 16 u + 8 h + j.
+      float x[16], top = -INFINITY;
+      bool whole = kb >= alo && kb + 32 <= ahi && kb + 32 <= hi;
+      // Pages that are not there: looked up again, a page (16 keys or more) per u.
+      bool there[2];
+#pragma unroll
+      for (int u = 0; u < 2; ++u) {
+        there[u] = kb + 16 * u < hi && page_of(table, kb + 16 * u, kv.shift, kv.pages) >= 0;
+        whole = whole && there[u];
+      }
+#pragma unroll
+      for (int i = 0; i < 16; ++i) {
+        const int key = kb + 16 * (i / 8) + 8 * h + i % 8;
+        x[i] = score(s[i] * back, pos - key);
+        if (!whole) x[i] = there[i / 8] && key <= pos && key >= first && key < hi ? x[i] : -INFINITY;
+        top = fmaxf(top, x[i]);
+      }
+      top = fmaxf(top, __shfl_xor(top, 32));
+      const float mn = fmaxf(m, top), ref = (mn == -INFINITY ? 0.0f : mn) - F::kLift;
+      const float alpha = m == mn ? 1.0f : __builtin_amdgcn_exp2f(m - mn);
+      m = mn;
+      float sum = 0.0f;
+#pragma unroll
+      for (int i = 0; i < 16; ++i) {
+        x[i] = __builtin_amdgcn_exp2f(x[i] - ref);
+        sum += x[i];
+      }
+      l = l * alpha + sum;
+      if (__any(alpha != 1.0f))
+#pragma unroll
+        for (int d = 0; d < HC; ++d) o[d] *= alpha;
+#pragma unroll
+      for (int u = 0; u < 2; ++u) {
+        float y[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) y[j] = x[8 * u + j];
+        u4 p[P];
+        F::parts(y, p);
+#pragma unroll
+        for (int d = 0; d < HC; ++d) {
+          u4 v[KP];
+#pragma unroll
+          for (int j = 0; j < KP; ++j) v[j] = vl[(((2 * sub + u) * HC + d) * KP + j) * 64 + lane];
+          o[d] = products<F>(v, p, o[d], [](u4 x, u4 y, f16v c) { return F::mma32(x, y, c); });
+        }
+      }
+    }
+    __syncthreads();
+  }
+  l += __shfl_xor(l, 32);
+  bool bad = !(fabsf(l) < INFINITY);
+#pragma unroll
+  for (int d = 0; d < HC; ++d)
+#pragma unroll
+    for (int i = 0; i < 16; ++i) bad = bad || !(fabsf(o[d][i]) < INFINITY);
+  if (r0 + col < rows) {
+    const size_t at = part_at(a, b, split, sp.q0 + tok, head);
+    float *out = a.out + (size_t)(sp.q0 + tok) * a.out_stride + (size_t)head * hd;
+    float inv = l == 0.0f ? 0.0f : 1.0f / l;
+    bool wide = vec;
+    if (splits > 1) {
+      out = sl.o + at * hd;
+      if (h == 0) sl.ml[at] = make_float2(m - F::kLift, l);
+      inv = 1.0f;
+      wide = true;
+    }
+#pragma unroll
+    for (int d = 0; d < HC; ++d)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int e = 32 * d + 8 * i + 4 * h;
+        if (e >= hd) continue;
+        const f4 y = f4{o[d][4 * i], o[d][4 * i + 1], o[d][4 * i + 2], o[d][4 * i + 3]} * inv;
+        if (wide)
+          *reinterpret_cast<f4 *>(out + e) = y;
+        else
+          for (int j = 0; j < 4; ++j) out[e + j] = y[j];
+      }
+  }
+  const uint64_t all = __ballot(bad);
+  for (uint32_t rest = (uint32_t)(all | all >> 32); rest; rest &= rest - 1) {
+    const int i = r0 + __builtin_ctz(rest);
+    if (i < rows)
+      redo_row(a, kv, b, sl, table, sp.q0 + i / per, kvh * per + i % per, base0 + i / per, lo, hi, split, splits);
+  }
+}
+
+// ------------------------------------------------------------------------ join --
+
+// Splits of a row joined: block (token x head, sequence); 32 lanes x 4 dimensions
+// twice over for heads past 128, eight shares of the splits.
+__global__ __launch_bounds__(256) void k_join(AttnArgs a, BatchView b, Splits sl, int nkv, int hd, bool vec) {
+  __shared__ float2 ms[8];
+  __shared__ f4 part[8][64];
+  const SeqSpan sp = seq_span(b, blockIdx.y);
+  const int j = blockIdx.x / a.heads, head = blockIdx.x % a.heads, per = a.heads / nkv;
+  if (j >= sp.nq) return;
+  const bool few = few_rows(sp.nq, per);
+  const int R = few ? kFewRows : kManyRows, len = few ? sl.few_len : sl.many_len;
+  const int splits = splits_of(tile_of(sp, (j * per + head % per) / R, R, per, a.window), len);
+  if (splits < 2) return;
+  const int lane = threadIdx.x & 31, share = threadIdx.x >> 5;
+  const size_t at = part_at(a, b, 0, sp.q0 + j, head), step = (size_t)b.tokens * a.heads;
+  float top = -INFINITY;
+  for (int s = threadIdx.x & 31; s < splits; s += 32) top = fmaxf(top, sl.ml[at + s * step].x);
+#pragma unroll
+  for (int d = 16; d; d >>= 1) top = fmaxf(top, __shfl_xor(top, d));
+  f4 o[2] = {f4{0, 0, 0, 0}, f4{0, 0, 0, 0}};
+  float l = 0.0f;
+  for (int s = share; s < splits; s += 8) {
+    const float2 x = sl.ml[at + s * step];
+    const float w = x.x == top ? 1.0f : exp2f(x.x - top);
+    l += w * x.y;
+    const float *p = sl.o + (at + s * step) * hd;
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+      if (4 * lane + 128 * i < hd) {
+        const f4 y = *reinterpret_cast<const f4 *>(p + 4 * lane + 128 * i);
+        o[i] += y * w;
+      }
+  }
+  if (lane == 0) ms[share].x = l;
+  part[share][lane] = o[0];
+  part[share][lane + 32] = o[1];
+  __syncthreads();
+  if (threadIdx.x >= 64 || 4 * (int)threadIdx.x >= hd) return;
+  f4 sum = part[0][threadIdx.x];
+  l = ms[0].x;
+#pragma unroll
+  for (int s = 1; s < 8; ++s) {
+    sum += part[s][threadIdx.x];
+    l += ms[s].x;
+  }
+  sum = l == 0.0f ? f4{0, 0, 0, 0} : sum * (1.0f / l);
+  float *out = a.out + (size_t)(sp.q0 + j) * a.out_stride + (size_t)head * hd + 4 * threadIdx.x;
+  if (vec)
+    *reinterpret_cast<f4 *>(out) = sum;
+  else
+    for (int i = 0; i < 4; ++i) out[i] = sum[i];
+}
+
+// --------------------------------------------------------------------- launch --
+
+// Splits of the key axis: as many as give the chip about `want` blocks, of whole
+// 128 positions, 256 at least.
+int split_len(size_t units, int keys, size_t want) {
+  const size_t n = std::max<size_t>(1, want / std::max<size_t>(units, 1));
+  const size_t len = (keys + n - 1) / n;
+  return (int)std::max<size_t>(256, (len + 127) / 128 * 128);
+}
+
+int most_keys(const BatchView &b, int window) {
+  const long long span = window > 0 ? (long long)window + b.max_q + 64 : b.max_kv;
+  return (int)std::max(1LL, std::min<long long>(b.max_kv, span));
+}
+
+struct Plan {
+  int few_len, many_len, few, many;  // split lengths and counts
+  bool use_few, use_many;
+};
+
+Plan plan_of(int nkv, int heads, int hd, const BatchView &b, int window, size_t work_bytes) {
+  Plan p;
+  const int per = heads / nkv, keys = most_keys(b, window);
+  const size_t row_bytes = (size_t)b.tokens * heads * (4 * (size_t)hd + 8);
+  const size_t fit = std::max<size_t>(1, work_bytes / row_bytes);
+  const size_t tiles = ((size_t)b.max_q * per + kManyRows - 1) / kManyRows;
+  p.use_few = true;
+  p.use_many = (size_t)b.max_q * per > kFewRows;
+  p.few_len = split_len((size_t)b.seqs * nkv, keys, 2048);
+  p.many_len = split_len((size_t)b.seqs * nkv * tiles, keys, 512);
+  auto count = [&](int &len) {
+    int n = (keys + 63 + len - 1) / len;
+    if ((size_t)n > fit) {
+      len = (int)(((keys + 63 + fit - 1) / fit + 127) / 128 * 128);
+      n = (keys + 63 + len - 1) / len;
+    }
+    return n;
+  };
+  p.few = count(p.few_len);
+  p.many = count(p.many_len);
+  return p;
+}
+
+template <class T, int HC>
+void launch_of(const AttnArgs &a, const LayerView<T> &kv, const BatchView &b, const Plan &p, const Splits &sl, bool vec,
+               hipStream_t s) {
+  if (p.use_many) {
+    const size_t tiles = ((size_t)b.max_q * (a.heads / kv.nkv) + kManyRows - 1) / kManyRows;
+    constexpr size_t lds = many_lds<T, HC>();
+    dynamic_lds<k_many<T, HC>>(lds);
+    k_many<T, HC><<<dim3((unsigned)(tiles * kv.nkv), p.many, b.seqs), 256, lds, s>>>(a, kv, b, sl, vec);
+  }
+  if (p.use_few) k_few<T, HC><<<dim3(p.few, kv.nkv, b.seqs), 256, 0, s>>>(a, kv, b, sl, vec);
+}
+
 }  // namespace
 
-size_t paged_attention_work(int, int, int, const BatchView &, int) { return 0; }
+size_t paged_attention_work(int nkv, int heads, int hd, const BatchView &b, int window) {
+  const Plan p = plan_of(nkv, heads, hd, b, window, SIZE_MAX);
+  const int most = std::max(p.few, p.use_many ? p.many : 1);
+  return most > 1 ? (size_t)most * b.tokens * heads * (4 * (size_t)hd + 8) : 0;
+}
 
 template <class T>
-void launch_paged_attention(const AttnArgs &a, const LayerView<T> &kv, const BatchView &b, void *, size_t,
-                            hipStream_t s) {
-  const size_t units = (size_t)b.max_q * a.heads;
-  k_rows<T><<<dim3((unsigned)((units + 3) / 4), b.seqs), 256, 0, s>>>(a, kv, b);
+void launch_paged_attention(const AttnArgs &a, const LayerView<T> &kv, const BatchView &b, void *work,
+                            size_t work_bytes, hipStream_t s) {
+  const Plan p = plan_of(kv.nkv, a.heads, kv.hd, b, a.window, work_bytes);
+  const int most = std::max(p.few, p.use_many ? p.many : 1);
+  Splits sl{p.few_len, p.many_len, most, static_cast<float *>(work), nullptr};
+  sl.ml = reinterpret_cast<float2 *>(sl.o + (size_t)most * b.tokens * a.heads * kv.hd);
+  const bool vec = ((uintptr_t)a.q | (uintptr_t)a.out) % 16 == 0 && a.q_stride % 4 == 0 && a.out_stride % 4 == 0;
+  switch ((kv.hd + 31) / 32) {
+    case 1: launch_of<T, 1>(a, kv, b, p, sl, vec, s); break;
+    case 2: launch_of<T, 2>(a, kv, b, p, sl, vec, s); break;
+    case 3: launch_of<T, 3>(a, kv, b, p, sl, vec, s); break;
+    case 4: launch_of<T, 4>(a, kv, b, p, sl, vec, s); break;
+    default: launch_of<T, 8>(a, kv, b, p, sl, vec, s); break;
+  }
+  if (most > 1)
+    k_join<<<dim3((unsigned)(b.max_q * a.heads), b.seqs), 256, 0, s>>>(a, b, sl, kv.nkv, kv.hd, vec);
 }
 
 template void launch_paged_attention<float>(const AttnArgs &, const LayerView<float> &, const BatchView &, void *, size_t,
