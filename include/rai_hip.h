@@ -417,9 +417,11 @@ int rai_paged_move_dev(const rai_pages *pages, const int32_t *src, const int32_t
  * [groups][take], best first, equal ones by beam, then logit, then token.  done (may be NULL)
  * [groups * beams]: a finished beam's only candidate is end_token at its present
  * score.  Scores are summed and compared in f64.  NaN logits count as -inf; a row
- * without a finite log-sum (all -inf, or +inf) and beams at -inf or NaN have no
- * candidates, and neither has a token at -inf; places past the last candidate
- * become -1, -1, -inf.  beams <= 64, take <= 64. */
+ * without a finite log-sum (all -inf, or +inf) and beams whose score is not finite
+ * have no candidates, and neither has a token at -inf; places past the last candidate
+ * become -1, -1, -inf.  beams <= 64, take <= 64, groups * beams <= 65535,
+ * vocab <= 2^30.  work: scratch of the call, rai_beam_select_workspace bytes,
+ * 16-byte aligned; calls that overlap in time need scratch of their own. */
 int rai_beam_select_workspace(size_t vocab, size_t groups, size_t beams, size_t take, size_t *bytes);
 int rai_beam_select_dev(const float *logits, size_t stride, size_t vocab, const float *scores, const uint8_t *done,
                         int32_t end_token, size_t groups, size_t beams, size_t take, int32_t *parent,

@@ -504,7 +504,7 @@ def _select(x, scores, done, end, beams, take):
             top = v.max()
             if not np.isfinite(top):
                 continue
-            t = base + (v - (top + np.log(np.exp(v - top).sum())))
+            t = base + (v - top - np.log(np.exp(v - top).sum()))  # a large top would swallow the logarithm
             best = np.lexsort((np.arange(vocab), -v))[:take]
             cand += [(-t[i], r, -v[i], int(i)) for i in best if v[i] > -np.inf]
         cand = sorted(cand)[:take]
