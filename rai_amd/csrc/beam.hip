@@ -32,7 +32,7 @@ size_t chunks_of(size_t vocab) { return (vocab + kChunkLogits - 1) / kChunkLogit
 struct Parts {
   double *sum;    // [row][chunk]
   float *top;     // [row][chunk]
-  uint64_t *key;  // [row][chunk][take]
+  uint64_t *key;  // [group][place][beam][chunk]
 };
 
 // Logit and token in one number that orders candidates of a row: larger logits
@@ -48,19 +48,18 @@ __device__ __forceinline__ float logit_of(uint64_t k) {
   return __uint_as_float(up & 0x80000000u ? up & 0x7fffffffu : ~up);
 }
 
-// exp(x - top) with the rounding of the difference and of its product with log2 e
-// carried along: only the half step of the exponential itself is left.
+// exp(x - top), x <= top: the product with log2 e carries its rounding along, so
+// that only the half steps of the difference and of the exponential are left.
 __device__ __forceinline__ float exp_near(float x, float top) {
-  constexpr float kLog2e = 1.4426950408889634f, kLow = 1.9259629911266175e-8f;
-  const float d = x - top, v = d - x, err = (x - (d - v)) - (top + v);
-  const float t = d * kLog2e;
-  if (t < -150.0f) return 0.0f;
-  const float low = fmaf(d, kLog2e, -t) + fmaf(d, kLow, err * kLog2e);
-  const float e = __builtin_amdgcn_exp2f(t);
-  return fmaf(e, low * 0.6931471805599453f, e);
+  constexpr float kLog2e = 1.4426950408889634f, kLow = 1.9259629911266175e-8f, kLn2 = 0.6931471805599453f;
+  const float d = fmaxf(x - top, -200.0f), t = d * kLog2e;
+  const float low = fmaf(d, kLow, fmaf(d, kLog2e, -t)), e = __builtin_amdgcn_exp2f(t);
+  return fmaf(e * kLn2, low, e);
 }
 
 __device__ __forceinline__ uint64_t shfl_of(uint64_t v, int d) { return __shfl_xor((unsigned long long)v, d); }
+__device__ __forceinline__ float shfl_of(float v, int d) { return __shfl_xor(v, d); }
+__device__ __forceinline__ double shfl_of(double v, int d) { return __shfl_xor(v, d); }
 
 // The smallest of the maxima of `groups` interleaved groups of the block's threads
 // (a power of two up to 64): at least `groups` of the block's values reach it, and
@@ -83,9 +82,13 @@ __device__ __forceinline__ V threshold(V v, int groups, V *red, Before better) {
   return v;
 }
 
-// Block (chunk, row): one pass over the logits, all of them in registers.
+constexpr int kList = 512;  // candidates of a chunk that are placed by counting
+
+// Block (chunk, row): one pass over the logits, all of them in registers.  Bound by
+// the vector instructions (about 15 a logit): the candidates are cut by their f32
+// value first, and by value and token only where too many are equal.
 __global__ __launch_bounds__(kThreads) void k_beam_chunk(BeamArgs a, Parts out, int groups, bool vec) {
-  __shared__ uint64_t list[kChunkLogits], red[kThreads];
+  __shared__ uint64_t list[kList], red[kThreads];
   __shared__ double sums[kThreads / 64];
   __shared__ float tops[kThreads / 64];
   __shared__ int count;
@@ -106,27 +109,26 @@ __global__ __launch_bounds__(kThreads) void k_beam_chunk(BeamArgs a, Parts out, 
       for (int j = 0; j < 4; ++j) v[4 * i + j] = e + j < a.vocab ? x[e + j] : -INFINITY;
     }
   }
+  auto token = [&](int i) { return base + 4 * (tid + kThreads * (i / 4)) + i % 4; };
   if (tid == 0) count = 0;
-  float top = -INFINITY;
-  uint64_t best = 0;
+  float mine = -INFINITY, top;
 #pragma unroll
-  for (int i = 0; i < kPer; ++i) {
-    top = fmaxf(top, v[i]);
-    best = max(best, key_of(v[i], base + 4 * (tid + kThreads * (i / 4)) + i % 4));
-  }
+  for (int i = 0; i < kPer; ++i) mine = fmaxf(mine, v[i]);
+  top = mine;
 #pragma unroll
   for (int d = 32; d; d >>= 1) top = fmaxf(top, __shfl_xor(top, d));
   if (lane == 0) tops[wave] = top;
-  const uint64_t least = threshold(best, groups, red, [](uint64_t p, uint64_t q) { return p > q; });
+  const float least = threshold(mine, groups, reinterpret_cast<float *>(red), [](float p, float q) { return p > q; });
 #pragma unroll
   for (int w = 0; w < kThreads / 64; ++w) top = fmaxf(top, tops[w]);
   // The candidates that can be among the best, in any order.
-  if (best >= least)
+  if (mine >= least && mine > -INFINITY)
 #pragma unroll
-    for (int i = 0; i < kPer; ++i) {
-      const uint64_t k = key_of(v[i], base + 4 * (tid + kThreads * (i / 4)) + i % 4);
-      if (k && k >= least) list[atomicAdd(&count, 1)] = k;
-    }
+    for (int i = 0; i < kPer; ++i)
+      if (v[i] >= least && v[i] > -INFINITY) {
+        const int n = atomicAdd(&count, 1);
+        if (n < kList) list[n] = key_of(v[i], token(i));
+      }
   float sum = 0.0f;
   if (fabsf(top) < INFINITY)
 #pragma unroll
@@ -140,114 +142,186 @@ __global__ __launch_bounds__(kThreads) void k_beam_chunk(BeamArgs a, Parts out, 
     out.sum[at] = (sums[0] + sums[1]) + (sums[2] + sums[3]);
     out.top[at] = top;
   }
+  // [group][place][beam][chunk]: the merge reads first places first.
+  const size_t lists = (size_t)a.beams * gridDim.x;
+  uint64_t *keys = out.key + (row / a.beams) * a.take * lists + row % a.beams * gridDim.x + blockIdx.x;
+  int n = count;
+  if (n > kList) {
+    uint64_t best = 0;
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) best = max(best, key_of(v[i], token(i)));
+    auto larger = [](uint64_t p, uint64_t q) { return p > q; };
+    const uint64_t cut = threshold(best, groups, red, larger);
+    if (tid == 0) count = 0;
+    __syncthreads();
+    if (best >= cut)
+#pragma unroll
+      for (int i = 0; i < kPer; ++i) {
+        const uint64_t k = key_of(v[i], token(i));
+        if (k && k >= cut) {
+          const int m = atomicAdd(&count, 1);
+          if (m < kList) list[m] = k;
+        }
+      }
+    __syncthreads();
+    n = count;
+    if (n > kList) {  // the best sit in a few threads: one after the other
+      uint64_t last = ~(uint64_t)0;
+      for (int p = 0; p < a.take; ++p) {
+        uint64_t next = 0;
+#pragma unroll
+        for (int i = 0; i < kPer; ++i) {
+          const uint64_t k = key_of(v[i], token(i));
+          if (k < last) next = max(next, k);
+        }
+        last = threshold(next, 1, red, larger);
+        if (tid == 0) keys[p * lists] = last;
+      }
+      return;
+    }
+  }
   // A candidate's place is the number of better ones.
-  const int n = count;
-  uint64_t *keys = out.key + at * a.take;
   for (int i = tid; i < n; i += kThreads) {
     const uint64_t k = list[i];
     int place = 0;
+#pragma unroll 8
     for (int j = 0; j < n; ++j) place += list[j] > k;
-    if (place < a.take) keys[place] = k;
+    if (place < a.take) keys[place * lists] = k;
   }
-  for (int i = n + tid; i < a.take; i += kThreads) keys[i] = 0;
+  for (int i = n + tid; i < a.take; i += kThreads) keys[i * lists] = 0;
 }
 
-// A candidate of a group and the order of the selection.
-struct Cand {
-  double score;  // -inf: none
-  uint64_t key;
-  int beam;
+// n / d for n < 2^31: the high half of n times ceil(2^(32 + s) / d) - 2^32, plus n.
+struct Div {
+  uint32_t d, m, s;
+  explicit Div(uint32_t by) : d(by), s(0) {
+    while ((uint64_t(1) << s) < by) ++s;
+    m = (uint32_t)(((uint64_t(1) << 32) * ((uint64_t(1) << s) - by)) / by + 1);
+  }
+  __device__ __forceinline__ uint32_t operator()(uint32_t n) const { return (__umulhi(m, n) + n) >> s; }
 };
-__device__ __forceinline__ bool before(const Cand &x, const Cand &y) {
-  if (x.score != y.score) return x.score > y.score;
-  return x.beam != y.beam ? x.beam < y.beam : x.key > y.key;
-}
-__device__ __forceinline__ Cand shfl_of(const Cand &c, int d) {
-  return {__shfl_xor(c.score, d), shfl_of(c.key, d), __shfl_xor(c.beam, d)};
-}
 
 constexpr int kBatch = 2048;  // candidates looked at in one go
 
 // One block per group: the chunks' lists merged, their first places first.  A
 // batch's candidates that reach the threshold (and the last of the best so far)
-// are placed by counting; a whole row of places without one ends the search.
-__global__ __launch_bounds__(kThreads) void k_beam_merge(BeamArgs a, Parts in, int chunks, int groups) {
+// are placed by counting.  Bound by the latency of its few dependent steps; `per`
+// threads (a power of two) share the chunks of a beam.
+__global__ __launch_bounds__(kThreads) void k_beam_merge(BeamArgs a, Parts in, int chunks, int groups, int per, Div by_lists,
+                                                         Div by_chunks) {
   __shared__ double base[64], less[64], tops[64], sc[kBatch + 64];
   __shared__ uint64_t key[kBatch + 64];
   __shared__ int bm[kBatch + 64];
-  __shared__ Cand red[kThreads], best[64];
+  __shared__ double red[kThreads], kept_sc[64];
+  __shared__ uint64_t kept_key[64];
+  __shared__ int kept_beam[64];
   __shared__ int count, have;
   const int g = blockIdx.x, tid = threadIdx.x;
+  const uint32_t lists = by_lists.d, all = lists * a.take;
+  const uint64_t *keys = in.key + (size_t)g * all;
+  constexpr int kN = kBatch / kThreads;
+  uint64_t k[kN];
+  auto load = [&](uint32_t from) {
+#pragma unroll
+    for (int i = 0; i < kN; ++i) {
+      const uint32_t e = from + tid + kThreads * i;
+      k[i] = e < all ? keys[e] : 0;
+    }
+  };
+  load(0);
   // Each beam's score (-inf where there is nothing to choose), its largest logit
   // and the logarithm of its sum: apart, since a large logit would swallow the others.
-  for (int b = tid; b < a.beams; b += kThreads) {
+  for (int b = tid / per; b < a.beams; b += kThreads / per) {
     const size_t row = (size_t)g * a.beams + b;
-    double s = a.scores[row], sum = 0.0;
-    float top = -INFINITY;
-    if (!(a.done && a.done[row])) {
-      for (int c = 0; c < chunks; ++c) top = fmaxf(top, in.top[row * chunks + c]);
-      for (int c = 0; c < chunks; ++c) {
+    const bool done = a.done && a.done[row];
+    float s = a.scores[row], top = -INFINITY;
+    double sum = 0.0;
+    if (!done) {
+      for (int c = tid & (per - 1); c < chunks; c += per) {
         const float t = in.top[row * chunks + c];
-        if (t > -INFINITY) sum += in.sum[row * chunks + c] * exp((double)t - (double)top);
+        const double w = in.sum[row * chunks + c];
+        if (!(t > -INFINITY)) continue;
+        const float m = fmaxf(top, t);
+        sum = sum * exp((double)top - (double)m) + w * exp((double)t - (double)m);
+        top = m;
       }
-      if (!(fabsf(top) < INFINITY)) s = -INFINITY;
+      for (int d = per >> 1; d; d >>= 1) {
+        const float t = __shfl_xor(top, d), m = fmaxf(top, t);
+        const double w = __shfl_xor(sum, d);
+        sum = (sum > 0.0 ? sum * exp((double)top - (double)m) : 0.0) + (w > 0.0 ? w * exp((double)t - (double)m) : 0.0);
+        top = m;
+      }
     }
-    tops[b] = top;
-    less[b] = log(sum);
-    base[b] = fabs(s) < INFINITY ? s : -(double)INFINITY;
+    if ((tid & (per - 1)) == 0) {
+      base[b] = fabsf(s) < INFINITY && (done || fabsf(top) < INFINITY) ? (double)s : -(double)INFINITY;
+      less[b] = log(sum);
+      tops[b] = done ? INFINITY : top;  // infinite: a finished beam
+    }
   }
   if (tid == 0) have = 0;
   __syncthreads();
-  const long long lists = (long long)a.beams * chunks, all = lists * a.take;
-  const Cand none{-(double)INFINITY, 0, 0};
-  for (long long from = 0; from < all; from += kBatch) {
-    Cand c[kBatch / kThreads], mine = none;
+  for (uint32_t from = 0; from < all; from += kBatch) {
+    double score[kN], mine = -INFINITY;
+    uint64_t ck[kN];
+    int beam[kN];
 #pragma unroll
-    for (int i = 0; i < kBatch / kThreads; ++i) {
-      const long long e = from + tid + kThreads * i;
-      c[i] = none;
-      if (e < all) {
-        const long long list = e % lists;
-        const int place = (int)(e / lists), beam = (int)(list / chunks), chunk = (int)(list % chunks);
-        const size_t row = (size_t)g * a.beams + beam;
-        c[i].beam = beam;
-        if (a.done && a.done[row]) {
-          if (place == 0 && chunk == 0) c[i] = {base[beam], key_of(0.0f, a.end_token), beam};
-        } else {
-          const uint64_t k = in.key[(row * chunks + chunk) * a.take + place];
-          if (k) c[i] = {base[beam] + ((double)logit_of(k) - tops[beam] - less[beam]), k, beam};
-        }
-        if (before(c[i], mine)) mine = c[i];
+    for (int i = 0; i < kN; ++i) {
+      const uint32_t e = from + tid + kThreads * i, list = e - by_lists(e) * lists;
+      beam[i] = (int)by_chunks(list);
+      ck[i] = k[i];
+      double s = base[beam[i]];
+      if (tops[beam[i]] == INFINITY) {
+        ck[i] = key_of(0.0f, a.end_token);
+        if (e >= lists || beam[i] * by_chunks.d != list) s = -INFINITY;
+      } else {
+        s += (double)logit_of(ck[i]) - tops[beam[i]] - less[beam[i]];
+        if (ck[i] == 0 || !(base[beam[i]] > -INFINITY)) s = -INFINITY;
       }
+      score[i] = e < all ? s : -INFINITY;
+      mine = fmax(mine, score[i]);
     }
+    load(from + kBatch < all ? from + kBatch : all);
     if (tid == 0) count = 0;
-    Cand least = threshold(mine, groups, red, before);
+    double least = threshold(mine, groups, red, [](double p, double q) { return p > q; });
     const int kept = have;
-    if (kept == a.take && before(best[kept - 1], least)) least = best[kept - 1];
+    if (kept == a.take) least = fmax(least, kept_sc[kept - 1]);
     int found = 0;
 #pragma unroll
-    for (int i = 0; i < kBatch / kThreads; ++i)
-      if (c[i].score > -INFINITY && !before(least, c[i])) {
+    for (int i = 0; i < kN; ++i)
+      if (score[i] > -INFINITY && score[i] >= least) {
         const int at = atomicAdd(&count, 1);
-        sc[at] = c[i].score;
-        key[at] = c[i].key;
-        bm[at] = c[i].beam;
+        sc[at] = score[i];
+        key[at] = ck[i];
+        bm[at] = beam[i];
         found = 1;
       }
     found = __syncthreads_or(found);
     if (found) {
       const int n = count + kept;
       if (tid < kept) {
-        sc[count + tid] = best[tid].score;
-        key[count + tid] = best[tid].key;
-        bm[count + tid] = best[tid].beam;
+        sc[count + tid] = kept_sc[tid];
+        key[count + tid] = kept_key[tid];
+        bm[count + tid] = kept_beam[tid];
       }
       __syncthreads();
       for (int i = tid; i < n; i += kThreads) {
-        const Cand x{sc[i], key[i], bm[i]};
-        int place = 0;
-        for (int j = 0; j < n; ++j) place += before(Cand{sc[j], key[j], bm[j]}, x);
-        if (place < a.take) best[place] = x;
+        const double s = sc[i];
+        const uint64_t x = key[i];
+        const int b = bm[i];
+        int place = 0, equal = 0;
+#pragma unroll 8
+        for (int j = 0; j < n; ++j) {
+          const double o = sc[j];
+          place += o > s;
+          equal += o == s;
+        }
+        if (equal > 1)
+          for (int j = 0; j < n; ++j) place += sc[j] == s && (bm[j] < b || (bm[j] == b && key[j] > x));
+        if (place < a.take) {
+          kept_sc[place] = s;
+          kept_key[place] = x;
+          kept_beam[place] = b;
+        }
       }
       if (tid == 0) have = min(n, a.take);
       __syncthreads();
@@ -259,9 +333,9 @@ __global__ __launch_bounds__(kThreads) void k_beam_merge(BeamArgs a, Parts in, i
   if (tid < a.take) {
     const size_t o = (size_t)g * a.take + tid;
     const bool ok = tid < have;
-    a.parent[o] = ok ? g * a.beams + best[tid].beam : -1;
-    a.token[o] = ok ? token_of(best[tid].key) : -1;
-    a.score[o] = ok ? (float)best[tid].score : -INFINITY;
+    a.parent[o] = ok ? g * a.beams + kept_beam[tid] : -1;
+    a.token[o] = ok ? token_of(kept_key[tid]) : -1;
+    a.score[o] = ok ? (float)kept_sc[tid] : -INFINITY;
   }
 }
 
@@ -313,7 +387,11 @@ int rai_beam_select_dev(const float *logits, size_t stride, size_t vocab, const 
     const bool vec = (uintptr_t)logits % 16 == 0 && stride % 4 == 0;
     hipStream_t s = (hipStream_t)stream;
     rai::k_beam_chunk<<<dim3((unsigned)chunks, (unsigned)rows), rai::kThreads, 0, s>>>(a, p, few, vec);
-    rai::k_beam_merge<<<(unsigned)groups, rai::kThreads, 0, s>>>(a, p, (int)chunks, few);
+    int per = 1;
+    while (per < 64 && (size_t)per < chunks && per * beams < rai::kThreads) per *= 2;
+    rai::k_beam_merge<<<(unsigned)groups, rai::kThreads, 0, s>>>(a, p, (int)chunks, few, per,
+                                                                 rai::Div((uint32_t)(beams * chunks)),
+                                                                 rai::Div((uint32_t)chunks));
     RAI_HIP_CHECK(hipGetLastError());
   });
 }

@@ -596,6 +596,19 @@ def test_beam_nothing_to_choose(rai, vocab):
     _check_beam(rai, x, scores, r.random(24) < 0.3, 1, 4, 8)
 
 
+@pytest.mark.parametrize("every,at", [(64, 5), (2, 1), (16, 0)])
+@pytest.mark.parametrize("take", [1, 16, 64])
+def test_beam_masked_in_a_pattern(rai, every, at, take):
+    """Masks that leave whole lanes of the selection empty, over chunks of which one is part filled."""
+    r = np.random.default_rng(every)
+    x = _normal(r, 4, 9001, 2.0)
+    x[:, np.arange(9001) // 4 % every == at] = -np.inf
+    x[1, 4096:] = -np.inf
+    x[2] = np.sort(x[2])
+    x[3] = -np.sort(-x[3])
+    _check_beam(rai, x, np.float32([-1, -2, -1.5, -1.25]), None, 0, 2, take)
+
+
 def test_beam_in_a_graph(rai):
     L, P = rai.lib(), ctypes.c_void_p
     groups, beams, vocab, take = 2, 4, 9000, 8
