@@ -98,15 +98,17 @@ __global__ __launch_bounds__(kThreads) void k_beam_chunk(BeamArgs a, Parts out, 
   const float *x = a.logits + row * a.stride;
   const int base = blockIdx.x * kChunkLogits;
   float v[kPer];
+  if (vec && base + kChunkLogits <= a.vocab) {
 #pragma unroll
-  for (int i = 0; i < kPer / 4; ++i) {
-    const int e = base + 4 * (tid + kThreads * i);
-    if (vec && e + 4 <= a.vocab) {
-      const float4 y = *reinterpret_cast<const float4 *>(x + e);
+    for (int i = 0; i < kPer / 4; ++i) {
+      const float4 y = *reinterpret_cast<const float4 *>(x + base + 4 * (tid + kThreads * i));
       v[4 * i] = y.x, v[4 * i + 1] = y.y, v[4 * i + 2] = y.z, v[4 * i + 3] = y.w;
-    } else {
+    }
+  } else {
 #pragma unroll
-      for (int j = 0; j < 4; ++j) v[4 * i + j] = e + j < a.vocab ? x[e + j] : -INFINITY;
+    for (int i = 0; i < kPer; ++i) {
+      const int e = base + 4 * (tid + kThreads * (i / 4)) + i % 4;
+      v[i] = e < a.vocab ? x[e] : -INFINITY;
     }
   }
   auto token = [&](int i) { return base + 4 * (tid + kThreads * (i / 4)) + i % 4; };
@@ -122,17 +124,22 @@ __global__ __launch_bounds__(kThreads) void k_beam_chunk(BeamArgs a, Parts out, 
 #pragma unroll
   for (int w = 0; w < kThreads / 64; ++w) top = fmaxf(top, tops[w]);
   // The candidates that can be among the best, in any order.
-  if (mine >= least && mine > -INFINITY)
+  uint32_t hits = 0;
+#pragma unroll
+  for (int i = 0; i < kPer; ++i) hits |= (v[i] >= least && v[i] > -INFINITY ? 1u : 0u) << i;
+  if (hits) {
+    int n = atomicAdd(&count, __popc(hits));
 #pragma unroll
     for (int i = 0; i < kPer; ++i)
-      if (v[i] >= least && v[i] > -INFINITY) {
-        const int n = atomicAdd(&count, 1);
+      if (hits >> i & 1) {
         if (n < kList) list[n] = key_of(v[i], token(i));
+        ++n;
       }
-  float sum = 0.0f;
+  }
+  float sum = 0.0f;  // -inf and NaN add nothing
   if (fabsf(top) < INFINITY)
 #pragma unroll
-    for (int i = 0; i < kPer; ++i) sum += v[i] > -INFINITY ? exp_near(v[i], top) : 0.0f;
+    for (int i = 0; i < kPer; ++i) sum += exp_near(v[i], top);
   double total = sum;
 #pragma unroll
   for (int d = 32; d; d >>= 1) total += __shfl_xor(total, d);
