@@ -315,11 +315,15 @@ __device__ __forceinline__ bool finite4(f4 x) {
 // At most 16 rows a kv head: one token of a sequence, or a verify batch.  Block
 // (split, kv head, sequence); the keys go to the waves 32 at a time, straight from
 // the pages into the operands (each is read once, so there is nothing to stage),
-// and the waves' softmaxes are joined in LDS.
+// and the waves' softmaxes are joined in LDS.  Bound by memory: the next step's
+// page ids, keys and values are on their way while a step is worked on, and f32
+// values go into the f32 instructions as they come (their rate is four times what
+// memory gives; cutting them costs more).
 template <class T, int HC>  // HC: head size in steps of 32, rounded up
 __global__ __launch_bounds__(256) void k_few(AttnArgs a, LayerView<T> kv, BatchView b, Splits sl, bool vec) {
   using F = Form<T>;
   constexpr int KP = F::KP, P = F::P, D = 2 * HC;
+  constexpr float kLift = sizeof(T) == 4 ? 0.0f : F::kLift;
   __shared__ float ml[2][4][16];
   __shared__ f4 part[2][D][64];
   __shared__ uint32_t bad_rows;
@@ -339,45 +343,50 @@ __global__ __launch_bounds__(256) void k_few(AttnArgs a, LayerView<T> kv, BatchV
   const int r = min(col, rows - 1), tok = r / per, head = kvh * per + r % per, pos = sp.n - sp.nq + tok;
   const int first = first_seen(pos, a.window);
   const Score score = score_of(a, head);
-  u4 q[HC][P];
-  float back;
+  constexpr bool kF32 = sizeof(T) == 4;
+  float qf[kF32 ? HC : 1][8];
+  u4 q[kF32 ? 1 : HC][P];
+  float back = a.scale;
   {
     const float *x = a.q + (size_t)(sp.q0 + tok) * a.q_stride + (size_t)head * hd;
-    float v[HC][8], most = 0.0f;
+    if constexpr (kF32) {
 #pragma unroll
-    for (int c = 0; c < HC; ++c) {
-      query8(x, 32 * c + 8 * g, hd, vec, v[c]);
+      for (int c = 0; c < HC; ++c) query8(x, 32 * c + 8 * g, hd, vec, qf[c]);
+    } else {
+      float v[HC][8], most = 0.0f;
 #pragma unroll
-      for (int i = 0; i < 8; ++i) most = fmaxf(most, fabsf(v[c][i]));
+      for (int c = 0; c < HC; ++c) {
+        query8(x, 32 * c + 8 * g, hd, vec, v[c]);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) most = fmaxf(most, fabsf(v[c][i]));
+      }
+      most = fmaxf(most, __shfl_xor(most, 16));
+      most = fmaxf(most, __shfl_xor(most, 32));
+      const int up = F::row_exponent(most);
+#pragma unroll
+      for (int c = 0; c < HC; ++c) {
+        if (up)
+#pragma unroll
+          for (int i = 0; i < 8; ++i) v[c][i] = ldexpf(v[c][i], up);
+        F::parts(v[c], q[c]);
+      }
+      back = ldexpf(a.scale, -up);
     }
-    most = fmaxf(most, __shfl_xor(most, 16));
-    most = fmaxf(most, __shfl_xor(most, 32));
-    const int up = F::row_exponent(most);
-#pragma unroll
-    for (int c = 0; c < HC; ++c) {
-      if (up)
-#pragma unroll
-        for (int i = 0; i < 8; ++i) v[c][i] = ldexpf(v[c][i], up);
-      F::parts(v[c], q[c]);
-    }
-    back = ldexpf(a.scale, -up);
   }
   f4 o[D];
 #pragma unroll
   for (int d = 0; d < D; ++d) o[d] = f4{0, 0, 0, 0};
   float m = -INFINITY, l = 0.0f;
-  for (int base = lo + 32 * wave; base < hi; base += 128) {
-    // Lane's key rows of the two score tiles: base + 8 (col / 4) + 4 t + col % 4;
-    // its keys in S^T and in V^T: base + 8 g ...
-    const int kk = base + 8 * (col >> 2), vk = base + 8 * g;
-    const int kpage = kk < hi ? page_of(table, kk, kv.shift, kv.pages) : -1;
-    const int vpage = vk < hi ? page_of(table, vk, kv.shift, kv.pages) : -1;
-    Raw<T> kr[2][HC], vr[D];
+  // Lane's key rows of the two score tiles: base + 8 (col / 4) + 4 t + col % 4; its
+  // keys in S^T and in V^T: base + 8 g ...
+  auto page_at = [&](int key) { return key < hi ? page_of(table, key, kv.shift, kv.pages) : -1; };
+  Raw<T> kr[2][HC], vr[D];
+  auto load_keys = [&](int kk, int page) {
 #pragma unroll
     for (int t = 0; t < 2; ++t) {
       const int key = kk + 4 * t + (col & 3);
-      const bool in = kpage >= 0 && key < hi && key >= seen;
-      const T *p = kv.k + key_at(max(kpage, 0), kvh, key & mask, kv.nkv, hd, kv.shift) + 8 * g;
+      const bool in = page >= 0 && key < hi && key >= seen;
+      const T *p = kv.k + key_at(max(page, 0), kvh, key & mask, kv.nkv, hd, kv.shift) + 8 * g;
 #pragma unroll
       for (int c = 0; c < HC; ++c) {
         if (in && 32 * c + 8 * g < hd)
@@ -386,25 +395,41 @@ __global__ __launch_bounds__(256) void k_few(AttnArgs a, LayerView<T> kv, BatchV
           kr[t][c].zero();
       }
     }
-    {
-      const T *p = kv.v + value_at(max(vpage, 0), kvh, vk & mask, kv.nkv, hd, kv.shift) + ((size_t)col << kv.shift);
+  };
+  auto load_values = [&](int vk, int page) {
+    const T *p = kv.v + value_at(max(page, 0), kvh, vk & mask, kv.nkv, hd, kv.shift) + ((size_t)col << kv.shift);
 #pragma unroll
-      for (int d = 0; d < D; ++d) {
-        if (vpage >= 0 && 16 * d + col < hd)
-          vr[d].load(p + ((size_t)(16 * d) << kv.shift));
-        else
-          vr[d].zero();
-      }
+    for (int d = 0; d < D; ++d) {
+      if (page >= 0 && 16 * d + col < hd)
+        vr[d].load(p + ((size_t)(16 * d) << kv.shift));
+      else
+        vr[d].zero();
     }
+  };
+  const int ko = 8 * (col >> 2), vo = 8 * g;
+  int base = lo + 32 * wave, vpage = page_at(base + vo), knext = page_at(base + 128 + ko), vnext = page_at(base + 128 + vo);
+  load_keys(base + ko, page_at(base + ko));
+  load_values(base + vo, vpage);
+  for (; base < hi; base += 128) {
+    const int vk = base + vo;
     f4 s[2] = {f4{0, 0, 0, 0}, f4{0, 0, 0, 0}};
 #pragma unroll
     for (int c = 0; c < HC; ++c)
+      if constexpr (kF32) {
 #pragma unroll
-      for (int t = 0; t < 2; ++t) {
-        u4 x[KP];
-        kr[t][c].parts(x);
-        s[t] = products<F>(x, q[c], s[t], [](u4 x, u4 y, f4 c) { return F::mma16(x, y, c); });
+        for (int e = 0; e < 8; ++e)
+#pragma unroll
+          for (int t = 0; t < 2; ++t)
+            s[t] = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(kr[t][c].v[e / 4][e % 4]), qf[c][e], s[t], 0, 0, 0);
+      } else {
+#pragma unroll
+        for (int t = 0; t < 2; ++t) {
+          u4 x[KP];
+          kr[t][c].parts(x);
+          s[t] = products<F>(x, q[c], s[t], [](u4 x, u4 y, f4 c) { return F::mma16(x, y, c); });
+        }
       }
+    if (base + 128 < hi) load_keys(base + 128 + ko, knext);  // while this step's softmax and values go on
     float x[8], top = -INFINITY;
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
@@ -415,7 +440,7 @@ __global__ __launch_bounds__(256) void k_few(AttnArgs a, LayerView<T> kv, BatchV
     }
     top = fmaxf(top, __shfl_xor(top, 16));
     top = fmaxf(top, __shfl_xor(top, 32));
-    const float mn = fmaxf(m, top), ref = (mn == -INFINITY ? 0.0f : mn) - F::kLift;
+    const float mn = fmaxf(m, top), ref = (mn == -INFINITY ? 0.0f : mn) - kLift;
     const float alpha = m == mn ? 1.0f : __builtin_amdgcn_exp2f(m - mn);
     m = mn;
     float sum = 0.0f;
@@ -428,17 +453,30 @@ __global__ __launch_bounds__(256) void k_few(AttnArgs a, LayerView<T> kv, BatchV
     if (__any(alpha != 1.0f))
 #pragma unroll
       for (int d = 0; d < D; ++d) o[d] *= alpha;
-    u4 p[P];
-    F::parts(x, p);
     // Slots that hold no key of these rows: whatever lies there stays out.
-    const bool edge = base < seen || base + 32 > hi;
+    if (base < seen || base + 32 > hi)
 #pragma unroll
-    for (int d = 0; d < D; ++d) {
-      if (edge) vr[d].keep(seen - vk, hi - vk);
-      u4 y[KP];
-      vr[d].parts(y);
-      o[d] = products<F>(y, p, o[d], [](u4 x, u4 y, f4 c) { return F::mma16(x, y, c); });
+      for (int d = 0; d < D; ++d) vr[d].keep(seen - vk, hi - vk);
+    if constexpr (kF32) {
+#pragma unroll
+      for (int e = 0; e < 8; ++e)
+#pragma unroll
+        for (int d = 0; d < D; ++d)
+          o[d] = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(vr[d].v[e / 4][e % 4]), x[e], o[d], 0, 0, 0);
+    } else {
+      u4 p[P];
+      F::parts(x, p);
+#pragma unroll
+      for (int d = 0; d < D; ++d) {
+        u4 y[KP];
+        vr[d].parts(y);
+        o[d] = products<F>(y, p, o[d], [](u4 x, u4 y, f4 c) { return F::mma16(x, y, c); });
+      }
     }
+    vpage = vnext;
+    if (base + 128 < hi) load_values(base + 128 + vo, vpage);
+    knext = page_at(base + 256 + ko);
+    vnext = page_at(base + 256 + vo);
   }
   // The four waves' softmaxes, then the four lane groups' shares of the sum.
   l += __shfl_xor(l, 16);
@@ -481,7 +519,7 @@ __global__ __launch_bounds__(256) void k_few(AttnArgs a, LayerView<T> kv, BatchV
       bool wide = vec;
       if (splits > 1) {
         out = sl.o + at * hd;
-        if (g == 0) sl.ml[at] = make_float2(top - F::kLift, sum);
+        if (g == 0) sl.ml[at] = make_float2(top - kLift, sum);
         inv = 1.0f;
         wide = true;
       }
@@ -819,7 +857,8 @@ int split_len(size_t units, int keys, size_t want) {
 }
 
 int most_keys(const BatchView &b, int window) {
-  const long long span = window > 0 ? (long long)window + b.max_q + 64 : b.max_kv;
+  // What a tile can read: its rows' windows, from a multiple of 64 on.
+  const long long span = window > 0 ? (long long)window + b.max_q + 63 : b.max_kv;
   return (int)std::max(1LL, std::min<long long>(b.max_kv, span));
 }
 
@@ -839,10 +878,10 @@ Plan plan_of(int nkv, int heads, int hd, const BatchView &b, int window, size_t 
   p.few_len = split_len((size_t)b.seqs * nkv, keys, 2048);
   p.many_len = split_len((size_t)b.seqs * nkv * tiles, keys, 512);
   auto count = [&](int &len) {
-    int n = (keys + 63 + len - 1) / len;
+    int n = (keys + len - 1) / len;
     if ((size_t)n > fit) {
-      len = (int)(((keys + 63 + fit - 1) / fit + 127) / 128 * 128);
-      n = (keys + 63 + len - 1) / len;
+      len = (int)(((keys + fit - 1) / fit + 127) / 128 * 128);
+      n = (keys + len - 1) / len;
     }
     return n;
   };
