@@ -291,6 +291,21 @@ struct Raw {
   }
 };
 
+// Values of a lane's keys in k_few: 16 bytes either way, eight of f16 or bf16, four
+// of f32.
+template <class T>
+struct Keys : Raw<T> {};
+template <>
+struct Keys<float> {
+  u4 v[1];
+  __device__ __forceinline__ void load(const float *p) { v[0] = *reinterpret_cast<const u4 *>(p); }
+  __device__ __forceinline__ void zero() { v[0] = u4{0, 0, 0, 0}; }
+  __device__ __forceinline__ void keep(int from, int to) {
+#pragma unroll
+    for (int e = 0; e < 4; ++e) v[0][e] = e >= from && e < to ? v[0][e] : 0u;
+  }
+};
+
 // Query values e .. e + 7 of a row (zero from hd on); `vec`: 16-byte loads fit.
 __device__ __forceinline__ void query8(const float *q, int e, int hd, bool vec, float (&x)[8]) {
   if (e >= hd) {
@@ -313,7 +328,7 @@ __device__ __forceinline__ bool finite4(f4 x) {
 // -------------------------------------------------------------------- few rows --
 
 // At most 16 rows a kv head: one token of a sequence, or a verify batch.  Block
-// (split, kv head, sequence); the keys go to the waves 32 at a time, straight from
+// (split, kv head, sequence); the keys go to the waves 32 at a time (16 of f32), straight from
 // the pages into the operands (each is read once, so there is nothing to stage),
 // and the waves' softmaxes are joined in LDS.  Bound by memory: the next step's
 // page ids, keys and values are on their way while a step is worked on, and f32
@@ -323,7 +338,9 @@ template <class T, int HC>  // HC: head size in steps of 32, rounded up
 __global__ __launch_bounds__(256) void k_few(AttnArgs a, LayerView<T> kv, BatchView b, Splits sl, bool vec) {
   using F = Form<T>;
   constexpr int KP = F::KP, P = F::P, D = 2 * HC;
-  constexpr float kLift = sizeof(T) == 4 ? 0.0f : F::kLift;
+  constexpr bool kF32 = sizeof(T) == 4;
+  constexpr int TK = kF32 ? 1 : 2, STEP = 16 * TK, N = 4 * TK;  // score tiles, keys of a step and of a lane
+  constexpr float kLift = kF32 ? 0.0f : F::kLift;
   __shared__ float ml[2][4][16];
   __shared__ f4 part[2][D][64];
   __shared__ uint32_t bad_rows;
@@ -343,7 +360,6 @@ __global__ __launch_bounds__(256) void k_few(AttnArgs a, LayerView<T> kv, BatchV
   const int r = min(col, rows - 1), tok = r / per, head = kvh * per + r % per, pos = sp.n - sp.nq + tok;
   const int first = first_seen(pos, a.window);
   const Score score = score_of(a, head);
-  constexpr bool kF32 = sizeof(T) == 4;
   float qf[kF32 ? HC : 1][8];
   u4 q[kF32 ? 1 : HC][P];
   float back = a.scale;
@@ -377,13 +393,14 @@ __global__ __launch_bounds__(256) void k_few(AttnArgs a, LayerView<T> kv, BatchV
 #pragma unroll
   for (int d = 0; d < D; ++d) o[d] = f4{0, 0, 0, 0};
   float m = -INFINITY, l = 0.0f;
-  // Lane's key rows of the two score tiles: base + 8 (col / 4) + 4 t + col % 4; its
-  // keys in S^T and in V^T: base + 8 g ...
+  // Lane's key rows of the score tiles: base + N (col / 4) + 4 t + col % 4; its keys
+  // in S^T and in V^T: base + N g ...
   auto page_at = [&](int key) { return key < hi ? page_of(table, key, kv.shift, kv.pages) : -1; };
-  Raw<T> kr[2][HC], vr[D];
+  Raw<T> kr[TK][HC];
+  Keys<T> vr[D];
   auto load_keys = [&](int kk, int page) {
 #pragma unroll
-    for (int t = 0; t < 2; ++t) {
+    for (int t = 0; t < TK; ++t) {
       const int key = kk + 4 * t + (col & 3);
       const bool in = page >= 0 && key < hi && key >= seen;
       const T *p = kv.k + key_at(max(page, 0), kvh, key & mask, kv.nkv, hd, kv.shift) + 8 * g;
@@ -406,33 +423,36 @@ __global__ __launch_bounds__(256) void k_few(AttnArgs a, LayerView<T> kv, BatchV
         vr[d].zero();
     }
   };
-  const int ko = 8 * (col >> 2), vo = 8 * g;
-  int base = lo + 32 * wave, vpage = page_at(base + vo), knext = page_at(base + 128 + ko), vnext = page_at(base + 128 + vo);
+  constexpr int ALL = 4 * STEP;  // a step of every wave
+  const int ko = N * (col >> 2), vo = N * g;
+  int base = lo + STEP * wave, vpage = page_at(base + vo), knext = page_at(base + ALL + ko), vnext = page_at(base + ALL + vo);
   load_keys(base + ko, page_at(base + ko));
   load_values(base + vo, vpage);
-  for (; base < hi; base += 128) {
+  for (; base < hi; base += ALL) {
     const int vk = base + vo;
-    f4 s[2] = {f4{0, 0, 0, 0}, f4{0, 0, 0, 0}};
+    f4 s[TK];
+#pragma unroll
+    for (int t = 0; t < TK; ++t) s[t] = f4{0, 0, 0, 0};
 #pragma unroll
     for (int c = 0; c < HC; ++c)
       if constexpr (kF32) {
 #pragma unroll
         for (int e = 0; e < 8; ++e)
 #pragma unroll
-          for (int t = 0; t < 2; ++t)
+          for (int t = 0; t < TK; ++t)
             s[t] = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(kr[t][c].v[e / 4][e % 4]), qf[c][e], s[t], 0, 0, 0);
       } else {
 #pragma unroll
-        for (int t = 0; t < 2; ++t) {
+        for (int t = 0; t < TK; ++t) {
           u4 x[KP];
           kr[t][c].parts(x);
           s[t] = products<F>(x, q[c], s[t], [](u4 x, u4 y, f4 c) { return F::mma16(x, y, c); });
         }
       }
-    if (base + 128 < hi) load_keys(base + 128 + ko, knext);  // while this step's softmax and values go on
-    float x[8], top = -INFINITY;
+    if (base + ALL < hi) load_keys(base + ALL + ko, knext);  // while this step's softmax and values go on
+    float x[N], top = -INFINITY;
 #pragma unroll
-    for (int e = 0; e < 8; ++e) {
+    for (int e = 0; e < N; ++e) {
       const int key = vk + e;
       const bool in = vpage >= 0 && key <= pos && key >= first && key < hi;
       x[e] = in ? score(s[e / 4][e % 4] * back, pos - key) : -INFINITY;
@@ -445,7 +465,7 @@ __global__ __launch_bounds__(256) void k_few(AttnArgs a, LayerView<T> kv, BatchV
     m = mn;
     float sum = 0.0f;
 #pragma unroll
-    for (int e = 0; e < 8; ++e) {
+    for (int e = 0; e < N; ++e) {
       x[e] = __builtin_amdgcn_exp2f(x[e] - ref);
       sum += x[e];
     }
@@ -454,12 +474,12 @@ __global__ __launch_bounds__(256) void k_few(AttnArgs a, LayerView<T> kv, BatchV
 #pragma unroll
       for (int d = 0; d < D; ++d) o[d] *= alpha;
     // Slots that hold no key of these rows: whatever lies there stays out.
-    if (base < seen || base + 32 > hi)
+    if (base < seen || base + STEP > hi)
 #pragma unroll
       for (int d = 0; d < D; ++d) vr[d].keep(seen - vk, hi - vk);
     if constexpr (kF32) {
 #pragma unroll
-      for (int e = 0; e < 8; ++e)
+      for (int e = 0; e < N; ++e)
 #pragma unroll
         for (int d = 0; d < D; ++d)
           o[d] = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(vr[d].v[e / 4][e % 4]), x[e], o[d], 0, 0, 0);
@@ -474,9 +494,9 @@ __global__ __launch_bounds__(256) void k_few(AttnArgs a, LayerView<T> kv, BatchV
       }
     }
     vpage = vnext;
-    if (base + 128 < hi) load_values(base + 128 + vo, vpage);
-    knext = page_at(base + 256 + ko);
-    vnext = page_at(base + 256 + vo);
+    if (base + ALL < hi) load_values(base + ALL + vo, vpage);
+    knext = page_at(base + 2 * ALL + ko);
+    vnext = page_at(base + 2 * ALL + vo);
   }
   // The four waves' softmaxes, then the four lane groups' shares of the sum.
   l += __shfl_xor(l, 16);
@@ -545,27 +565,31 @@ __global__ __launch_bounds__(256) void k_few(AttnArgs a, LayerView<T> kv, BatchV
 // ------------------------------------------------------------------- many rows --
 
 // Chunks of a prompt.  Block (row tile x kv head, split, sequence): each of four
-// waves has 32 rows, and a stage of keys and values passes through LDS for all of
+// waves has 32 rows, and stages of 32 keys and values pass through LDS for all of
 // them, lying there operand by operand (lane after lane, so that reads are linear
-// and f32 values are cut into their parts once for the block).  The next stage's
-// values come from the pages while a stage is worked on.
+// and f32 values are cut into their parts once for the block).  While a stage is
+// worked on, the next one's keys and then its values come from the pages through
+// the same few registers: two blocks share a CU, one's softmax beside the other's
+// products.  Two buffers of keys and of values, one of f32 values (LDS).
+constexpr int kStage = 32;
 template <class T>
-constexpr int kStage = sizeof(T) == 4 ? 32 : 64;
+constexpr int kValueBufs = sizeof(T) == 4 ? 1 : 2;
 
 template <class T, int HC>
 constexpr size_t many_lds() {
-  return (size_t)2 * kStage<T> * HC * 32 * 2 * Form<T>::KP;
+  return (size_t)(2 + kValueBufs<T>) * kStage * HC * 32 * 2 * Form<T>::KP;
 }
 
 // Row of a 32 x 32 operand that holds key k of its 32.
 __device__ __forceinline__ int key_row(int k) { return (k & 16) + 2 * (k & 4) + ((k & 8) >> 1) + (k & 3); }
 
 template <class T, int HC>
-__global__ __launch_bounds__(256) void k_many(AttnArgs a, LayerView<T> kv, BatchView b, Splits sl, bool vec) {
+__global__ __launch_bounds__(256, HC <= 4 ? 2 : 1) void k_many(AttnArgs a, LayerView<T> kv, BatchView b, Splits sl, bool vec) {
   using F = Form<T>;
-  constexpr int KP = F::KP, P = F::P, S = kStage<T>, SUB = S / 32, KS = 2 * HC, UNITS = S * HC * 4, U = (UNITS + 255) / 256;
+  constexpr int KP = F::KP, P = F::P, S = kStage, KS = 2 * HC, UNITS = S * HC * 4, U = (UNITS + 255) / 256;
+  constexpr int BUF = KS * KP * 64;  // a stage of keys, or of values
   extern __shared__ __align__(16) uint8_t lds[];
-  u4 *kl = reinterpret_cast<u4 *>(lds), *vl = kl + SUB * KS * KP * 64;
+  u4 *kl = reinterpret_cast<u4 *>(lds), *vl = kl + 2 * BUF;
   const int seq = blockIdx.z, split = blockIdx.y, per = a.heads / kv.nkv, hd = kv.hd;
   const SeqSpan sp = seq_span(b, seq);
   const int rows = sp.nq * per, tiles = (rows + kManyRows - 1) / kManyRows;
@@ -626,88 +650,101 @@ __global__ __launch_bounds__(256) void k_many(AttnArgs a, LayerView<T> kv, Batch
 
   // Unit u of a stage's keys: 16 keys x 4 chunks of 8 dimensions per 64 units; of
   // its values: 16 dimensions x 4 chunks of 8 keys.
-  Raw<T> kr[U], vr[U];
+  Raw<T> raw[U];
   auto key_unit = [](int u, int &key, int &chunk) {
-    key = (u & 15) + 16 * ((u >> 6) % (S / 16));
-    chunk = ((u >> 4) & 3) + 4 * ((u >> 6) / (S / 16));
+    key = (u & 15) + 16 * ((u >> 6) & 1);
+    chunk = ((u >> 4) & 3) + 4 * (u >> 7);
   };
   auto value_unit = [](int u, int &d, int &chunk) {
-    d = (u & 15) + 16 * ((u >> 6) % (2 * HC));
-    chunk = ((u >> 4) & 3) + 4 * ((u >> 6) / (2 * HC));
+    d = (u & 15) + 16 * (u >> 6);
+    chunk = (u >> 4) & 3;
   };
-  auto load = [&](int base) {
+  auto mine = [&](int i) { return UNITS % 256 == 0 || tid + 256 * i < UNITS; };
+  auto load_keys = [&](int base) {
 #pragma unroll
     for (int i = 0; i < U; ++i) {
       int key, chunk;
       key_unit(tid + 256 * i, key, chunk);
       key += base;
       const int page = key < hi ? page_of(table, key, kv.shift, kv.pages) : -1;
-      if (page >= 0 && key >= seen && 8 * chunk < hd && (UNITS % 256 == 0 || tid + 256 * i < UNITS))
-        kr[i].load(kv.k + key_at(page, kvh, key & mask, kv.nkv, hd, kv.shift) + 8 * chunk);
+      if (page >= 0 && key >= seen && 8 * chunk < hd && mine(i))
+        raw[i].load(kv.k + key_at(page, kvh, key & mask, kv.nkv, hd, kv.shift) + 8 * chunk);
       else
-        kr[i].zero();
+        raw[i].zero();
     }
+  };
+  auto put_keys = [&](u4 *buf) {
+#pragma unroll
+    for (int i = 0; i < U; ++i) {
+      if (!mine(i)) break;
+      int key, chunk;
+      key_unit(tid + 256 * i, key, chunk);
+      u4 x[KP];
+      raw[i].parts(x);
+      u4 *to = buf + (chunk >> 1) * KP * 64 + (chunk & 1) * 32 + key_row(key);
+#pragma unroll
+      for (int j = 0; j < KP; ++j) to[j * 64] = x[j];
+    }
+  };
+  auto load_values = [&](int base) {
 #pragma unroll
     for (int i = 0; i < U; ++i) {
       int d, chunk;
       value_unit(tid + 256 * i, d, chunk);
       const int key = base + 8 * chunk;
       const int page = key < hi ? page_of(table, key, kv.shift, kv.pages) : -1;
-      if (page >= 0 && d < hd && (UNITS % 256 == 0 || tid + 256 * i < UNITS))
-        vr[i].load(kv.v + value_at(page, kvh, key & mask, kv.nkv, hd, kv.shift) + ((size_t)d << kv.shift));
+      if (page >= 0 && d < hd && mine(i))
+        raw[i].load(kv.v + value_at(page, kvh, key & mask, kv.nkv, hd, kv.shift) + ((size_t)d << kv.shift));
       else
-        vr[i].zero();
+        raw[i].zero();
     }
   };
-  auto put = [&](int base) {
+  auto put_values = [&](u4 *buf, int base) {
     const bool edge = base < seen || base + S > hi;
 #pragma unroll
     for (int i = 0; i < U; ++i) {
-      int key, chunk;
-      key_unit(tid + 256 * i, key, chunk);
-      if (UNITS % 256 && tid + 256 * i >= UNITS) break;
-      u4 x[KP];
-      kr[i].parts(x);
-      u4 *to = kl + ((key >> 5) * KS + (chunk >> 1)) * KP * 64 + (chunk & 1) * 32 + key_row(key & 31);
-#pragma unroll
-      for (int j = 0; j < KP; ++j) to[j * 64] = x[j];
-    }
-#pragma unroll
-    for (int i = 0; i < U; ++i) {
+      if (!mine(i)) break;
       int d, chunk;
       value_unit(tid + 256 * i, d, chunk);
-      if (UNITS % 256 && tid + 256 * i >= UNITS) break;
-      if (edge) vr[i].keep(seen - base - 8 * chunk, hi - base - 8 * chunk);
+      if (edge) raw[i].keep(seen - base - 8 * chunk, hi - base - 8 * chunk);
       u4 x[KP];
-      vr[i].parts(x);
-      u4 *to = vl + ((chunk >> 1) * HC + (d >> 5)) * KP * 64 + (chunk & 1) * 32 + (d & 31);
+      raw[i].parts(x);
+      u4 *to = buf + ((chunk >> 1) * HC + (d >> 5)) * KP * 64 + (chunk & 1) * 32 + (d & 31);
 #pragma unroll
       for (int j = 0; j < KP; ++j) to[j * 64] = x[j];
     }
   };
 
-  load(lo);
-  for (int base = lo; base < hi; base += S) {
-    put(base);
+  load_keys(lo);
+  put_keys(kl);
+  load_values(lo);
+  put_values(vl, lo);
+  int cur = 0;
+  for (int kb = lo; kb < hi; kb += S, cur ^= 1) {
+    const bool more = kb + S < hi, work = !idle && kb < whi && kb + S > wlo;
+    const u4 *kbuf = kl + cur * BUF, *vbuf = vl + (kValueBufs<T> > 1 ? cur : 0) * BUF;
     __syncthreads();
-    if (base + S < hi) load(base + S);
-#pragma unroll
-    for (int sub = 0; sub < SUB; ++sub) {
-      const int kb = base + 32 * sub;
-      if (idle || kb >= whi || kb + 32 <= wlo) continue;
-      f16v s;
+    if (more) load_keys(kb + S);
+    f16v s;
+    if (work) {
 #pragma unroll
       for (int i = 0; i < 16; ++i) s[i] = 0.0f;
 #pragma unroll
       for (int c = 0; c < KS; ++c) {
         u4 x[KP];
 #pragma unroll
-        for (int j = 0; j < KP; ++j) x[j] = kl[((sub * KS + c) * KP + j) * 64 + lane];
+        for (int j = 0; j < KP; ++j) x[j] = kbuf[(c * KP + j) * 64 + lane];
         s = products<F>(x, q[c], s, [](u4 x, u4 y, f16v c) { return F::mma32(x, y, c); });
       }
+    }
+    if (more) {
+      put_keys(kl + (cur ^ 1) * BUF);
+      load_values(kb + S);
+    }
+    if (work) {
       // Register 8 u + j of a lane is key kb + 16 u + 8 h + j.
       float x[16], top = -INFINITY;
-      bool whole = kb >= alo && kb + 32 <= ahi && kb + 32 <= hi;
+      bool whole = kb >= alo && kb + S <= ahi && kb + S <= hi;
       // Pages that are not there: looked up again, a page (16 keys or more) per u.
       bool there[2];
 #pragma unroll
@@ -716,12 +753,15 @@ __global__ __launch_bounds__(256) void k_many(AttnArgs a, LayerView<T> kv, Batch
         whole = whole && there[u];
       }
 #pragma unroll
-      for (int i = 0; i < 16; ++i) {
-        const int key = kb + 16 * (i / 8) + 8 * h + i % 8;
-        x[i] = score(s[i] * back, pos - key);
-        if (!whole) x[i] = there[i / 8] && key <= pos && key >= first && key < hi ? x[i] : -INFINITY;
-        top = fmaxf(top, x[i]);
-      }
+      for (int i = 0; i < 16; ++i) x[i] = score(s[i] * back, pos - (kb + 16 * (i / 8) + 8 * h + i % 8));
+      if (!whole)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+          const int key = kb + 16 * (i / 8) + 8 * h + i % 8;
+          x[i] = there[i / 8] && key <= pos && key >= first && key < hi ? x[i] : -INFINITY;
+        }
+#pragma unroll
+      for (int i = 0; i < 16; ++i) top = fmaxf(top, x[i]);
       top = fmaxf(top, __shfl_xor(top, 32));
       const float mn = fmaxf(m, top), ref = (mn == -INFINITY ? 0.0f : mn) - F::kLift;
       const float alpha = m == mn ? 1.0f : __builtin_amdgcn_exp2f(m - mn);
@@ -747,12 +787,13 @@ __global__ __launch_bounds__(256) void k_many(AttnArgs a, LayerView<T> kv, Batch
         for (int d = 0; d < HC; ++d) {
           u4 v[KP];
 #pragma unroll
-          for (int j = 0; j < KP; ++j) v[j] = vl[(((2 * sub + u) * HC + d) * KP + j) * 64 + lane];
+          for (int j = 0; j < KP; ++j) v[j] = vbuf[((u * HC + d) * KP + j) * 64 + lane];
           o[d] = products<F>(v, p, o[d], [](u4 x, u4 y, f16v c) { return F::mma32(x, y, c); });
         }
       }
     }
-    __syncthreads();
+    if (kValueBufs<T> == 1) __syncthreads();
+    if (more) put_values(vl + (kValueBufs<T> > 1 ? cur ^ 1 : 0) * BUF, kb + S);
   }
   l += __shfl_xor(l, 32);
   bool bad = !(fabsf(l) < INFINITY);
@@ -794,56 +835,62 @@ __global__ __launch_bounds__(256) void k_many(AttnArgs a, LayerView<T> kv, Batch
 
 // ------------------------------------------------------------------------ join --
 
-// Splits of a row joined: block (token x head, sequence); 32 lanes x 4 dimensions
-// twice over for heads past 128, eight shares of the splits.
-__global__ __launch_bounds__(256) void k_join(AttnArgs a, BatchView b, Splits sl, int nkv, int hd, bool vec) {
-  __shared__ float2 ms[8];
+// Splits of a row joined: 32 lanes x 4 dimensions (twice over for heads past 128)
+// by `shares` (1 to 8, a power of two) that take the splits in turn; a block has 8 /
+// shares rows.  Block (rows, sequence).
+__global__ __launch_bounds__(256) void k_join(AttnArgs a, BatchView b, Splits sl, int nkv, int hd, int shares, bool vec) {
+  __shared__ float ls[8];
   __shared__ f4 part[8][64];
   const SeqSpan sp = seq_span(b, blockIdx.y);
-  const int j = blockIdx.x / a.heads, head = blockIdx.x % a.heads, per = a.heads / nkv;
-  if (j >= sp.nq) return;
+  const int lane = threadIdx.x & 31, w = threadIdx.x >> 5, share = w & (shares - 1);
+  const int unit = blockIdx.x * (8 / shares) + w / shares, j = unit / a.heads, head = unit % a.heads, per = a.heads / nkv;
   const bool few = few_rows(sp.nq, per);
   const int R = few ? kFewRows : kManyRows, len = few ? sl.few_len : sl.many_len;
-  const int splits = splits_of(tile_of(sp, (j * per + head % per) / R, R, per, a.window), len);
-  if (splits < 2) return;
-  const int lane = threadIdx.x & 31, share = threadIdx.x >> 5;
-  const size_t at = part_at(a, b, 0, sp.q0 + j, head), step = (size_t)b.tokens * a.heads;
-  float top = -INFINITY;
-  for (int s = threadIdx.x & 31; s < splits; s += 32) top = fmaxf(top, sl.ml[at + s * step].x);
-#pragma unroll
-  for (int d = 16; d; d >>= 1) top = fmaxf(top, __shfl_xor(top, d));
+  const int splits = j < sp.nq ? splits_of(tile_of(sp, (j * per + head % per) / R, R, per, a.window), len) : 0;
+  const size_t at = part_at(a, b, 0, sp.q0 + min(j, max(sp.nq - 1, 0)), head), step = (size_t)b.tokens * a.heads;
   f4 o[2] = {f4{0, 0, 0, 0}, f4{0, 0, 0, 0}};
   float l = 0.0f;
-  for (int s = share; s < splits; s += 8) {
-    const float2 x = sl.ml[at + s * step];
-    const float w = x.x == top ? 1.0f : exp2f(x.x - top);
-    l += w * x.y;
-    const float *p = sl.o + (at + s * step) * hd;
+  if (splits > 1) {
+    float top = -INFINITY;
+    for (int s = lane; s < splits; s += 32) top = fmaxf(top, sl.ml[at + s * step].x);
 #pragma unroll
-    for (int i = 0; i < 2; ++i)
-      if (4 * lane + 128 * i < hd) {
-        const f4 y = *reinterpret_cast<const f4 *>(p + 4 * lane + 128 * i);
-        o[i] += y * w;
-      }
-  }
-  if (lane == 0) ms[share].x = l;
-  part[share][lane] = o[0];
-  part[share][lane + 32] = o[1];
-  __syncthreads();
-  if (threadIdx.x >= 64 || 4 * (int)threadIdx.x >= hd) return;
-  f4 sum = part[0][threadIdx.x];
-  l = ms[0].x;
+    for (int d = 16; d; d >>= 1) top = fmaxf(top, __shfl_xor(top, d));
+#pragma unroll 4
+    for (int s = share; s < splits; s += shares) {
+      const float2 x = sl.ml[at + s * step];
+      const float weight = x.x == top ? 1.0f : __builtin_amdgcn_exp2f(x.x - top);
+      l += weight * x.y;
+      const float *p = sl.o + (at + s * step) * hd;
 #pragma unroll
-  for (int s = 1; s < 8; ++s) {
-    sum += part[s][threadIdx.x];
-    l += ms[s].x;
+      for (int i = 0; i < 2; ++i)
+        if (4 * lane + 128 * i < hd) o[i] += *reinterpret_cast<const f4 *>(p + 4 * lane + 128 * i) * weight;
+    }
   }
-  sum = l == 0.0f ? f4{0, 0, 0, 0} : sum * (1.0f / l);
-  float *out = a.out + (size_t)(sp.q0 + j) * a.out_stride + (size_t)head * hd + 4 * threadIdx.x;
-  if (vec)
-    *reinterpret_cast<f4 *>(out) = sum;
-  else
-    for (int i = 0; i < 4; ++i) out[i] = sum[i];
+  if (shares > 1) {
+    if (lane == 0) ls[w] = l;
+    part[w][lane] = o[0];
+    part[w][lane + 32] = o[1];
+    __syncthreads();
+    if (share) return;
+    for (int s = 1; s < shares; ++s) {
+      l += ls[w + s];
+      o[0] += part[w + s][lane];
+      o[1] += part[w + s][lane + 32];
+    }
+  }
+  if (splits < 2) return;
+  const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+  float *out = a.out + (size_t)(sp.q0 + j) * a.out_stride + (size_t)head * hd;
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    const int e = 4 * lane + 128 * i;
+    if (e >= hd) continue;
+    const f4 y = o[i] * inv;
+    if (vec)
+      *reinterpret_cast<f4 *>(out + e) = y;
+    else
+      for (int k = 0; k < 4; ++k) out[e + k] = y[k];
+  }
 }
 
 // --------------------------------------------------------------------- launch --
@@ -925,8 +972,13 @@ void launch_paged_attention(const AttnArgs &a, const LayerView<T> &kv, const Bat
     case 4: launch_of<T, 4>(a, kv, b, p, sl, vec, s); break;
     default: launch_of<T, 8>(a, kv, b, p, sl, vec, s); break;
   }
-  if (most > 1)
-    k_join<<<dim3((unsigned)(b.max_q * a.heads), b.seqs), 256, 0, s>>>(a, b, sl, kv.nkv, kv.hd, vec);
+  if (most > 1) {
+    int shares = 1;
+    while (shares < 8 && 4 * shares < most) shares *= 2;
+    const int rows = 8 / shares;
+    k_join<<<dim3((unsigned)((b.max_q * a.heads + rows - 1) / rows), b.seqs), 256, 0, s>>>(a, b, sl, kv.nkv, kv.hd, shares,
+                                                                                           vec);
+  }
 }
 
 template void launch_paged_attention<float>(const AttnArgs &, const LayerView<float> &, const BatchView &, void *, size_t,
