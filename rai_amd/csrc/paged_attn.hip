@@ -119,7 +119,7 @@ __device__ __forceinline__ size_t part_at(const AttnArgs &a, const BatchView &b,
 // of the output.  Keys that are not there or masked are not read into the sums at
 // all, whatever they hold.  m is in the log2 domain.
 template <class T>
-__device__ void wave_row(const AttnArgs &a, const LayerView<T> &kv, const int *table, int head, const float *q, int pos,
+__device__ __forceinline__ void wave_row(const AttnArgs &a, const LayerView<T> &kv, const int *table, int head, const float *q, int pos,
                          int lo, int hi, float &m, float &l, float (&o)[4]) {
   const int lane = threadIdx.x & 63, hd = kv.hd, kvh = head / (a.heads / kv.nkv), mask = (1 << kv.shift) - 1;
   const Score score = score_of(a, head);
@@ -159,7 +159,7 @@ __device__ void wave_row(const AttnArgs &a, const LayerView<T> &kv, const int *t
 
 // A row's result again, from its own keys of positions lo .. hi - 1 (of the split).
 template <class T>
-__device__ __noinline__ void redo_row(const AttnArgs &a, const LayerView<T> &kv, const BatchView &b, const Splits &sl,
+__device__ __forceinline__ void redo_row(const AttnArgs &a, const LayerView<T> &kv, const BatchView &b, const Splits &sl,
                                       const int *table, int row, int head, int pos, int lo, int hi, int split,
                                       int splits) {
   const int lane = threadIdx.x & 63;
