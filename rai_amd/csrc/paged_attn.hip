@@ -291,6 +291,15 @@ struct Raw {
   }
 };
 
+// A lane's eight values of an operand in LDS (f32: in two halves of 64 lanes).
+template <class T>
+__device__ __forceinline__ void fetch(const u4 *at, u4 (&x)[Form<T>::KP]) {
+  Raw<T> r;
+#pragma unroll
+  for (int i = 0; i < (int)sizeof(T) / 2; ++i) r.v[i] = at[64 * i];
+  r.parts(x);
+}
+
 // Values of a lane's keys in k_few: 16 bytes either way, eight of f16 or bf16, four
 // of f32.
 template <class T>
@@ -566,28 +575,35 @@ __global__ __launch_bounds__(256) void k_few(AttnArgs a, LayerView<T> kv, BatchV
 
 // Chunks of a prompt.  Block (row tile x kv head, split, sequence): each of four
 // waves has 32 rows, and stages of 32 keys and values pass through LDS for all of
-// them, lying there operand by operand (lane after lane, so that reads are linear
-// and f32 values are cut into their parts once for the block).  While a stage is
-// worked on, the next one's keys and then its values come from the pages through
-// the same few registers: two blocks share a CU, one's softmax beside the other's
-// products.  Two buffers of keys and of values, one of f32 values (LDS).
+// them, as they are in the pages but dealt operand by operand, lane after lane (so
+// that reads are linear).  They get there by DMA, a stage ahead and without a
+// register.  Two blocks share a CU, one's softmax beside the other's products.
 constexpr int kStage = 32;
-template <class T>
-constexpr int kValueBufs = sizeof(T) == 4 ? 1 : 2;
 
 template <class T, int HC>
 constexpr size_t many_lds() {
-  return (size_t)(2 + kValueBufs<T>) * kStage * HC * 32 * 2 * Form<T>::KP;
+  return (size_t)2 * 2 * kStage * HC * 32 * sizeof(T);
 }
 
-// Row of a 32 x 32 operand that holds key k of its 32.
-__device__ __forceinline__ int key_row(int k) { return (k & 16) + 2 * (k & 4) + ((k & 8) >> 1) + (k & 3); }
+typedef __attribute__((address_space(3))) void lds_void;
+typedef const __attribute__((address_space(1))) void global_void;
+
+// Eight cache values of each lane (p: the lane's) to a 64-lane operand in LDS: f32
+// in two halves.
+template <class T>
+__device__ __forceinline__ void dma(const T *p, u4 *to) {
+  __builtin_amdgcn_global_load_lds((global_void *)p, (lds_void *)to, 16, 0, 0);
+  if constexpr (sizeof(T) == 4) __builtin_amdgcn_global_load_lds((global_void *)(p + 4), (lds_void *)(to + 64), 16, 0, 0);
+}
+
+// Key of its 32 that row r of a 32 x 32 operand holds.
+__device__ __forceinline__ int row_key(int r) { return (r & 16) + 2 * (r & 4) + ((r & 8) >> 1) + (r & 3); }
 
 template <class T, int HC>
 __global__ __launch_bounds__(256, HC <= 4 ? 2 : 1) void k_many(AttnArgs a, LayerView<T> kv, BatchView b, Splits sl, bool vec) {
   using F = Form<T>;
-  constexpr int KP = F::KP, P = F::P, S = kStage, KS = 2 * HC, UNITS = S * HC * 4, U = (UNITS + 255) / 256;
-  constexpr int BUF = KS * KP * 64;  // a stage of keys, or of values
+  constexpr int KP = F::KP, P = F::P, S = kStage, KS = 2 * HC;
+  constexpr int OP = 64 * sizeof(T) / 2, BUF = KS * OP;  // an operand, and a stage of keys or of values, in 16 bytes
   extern __shared__ __align__(16) uint8_t lds[];
   u4 *kl = reinterpret_cast<u4 *>(lds), *vl = kl + 2 * BUF;
   const int seq = blockIdx.z, split = blockIdx.y, per = a.heads / kv.nkv, hd = kv.hd;
@@ -618,6 +634,7 @@ __global__ __launch_bounds__(256, HC <= 4 ? 2 : 1) void k_many(AttnArgs a, Layer
   float back;
   {
     const float *x = a.q + (size_t)(sp.q0 + tok) * a.q_stride + (size_t)head * hd;
+    const float sign = a.scale < 0.0f ? -1.0f : 1.0f;  // the scale is positive from here on
     float most = 0.0f;
     int up = 0;
     if (F::kLift != 0.0f) {  // f16
@@ -634,13 +651,15 @@ __global__ __launch_bounds__(256, HC <= 4 ? 2 : 1) void k_many(AttnArgs a, Layer
     for (int c = 0; c < KS; ++c) {
       float v[8];
       query8(x, 16 * c + 8 * h, hd, vec, v);
-      if (F::kLift != 0.0f)
 #pragma unroll
-        for (int i = 0; i < 8; ++i) v[i] = ldexpf(v[i], up);
+      for (int i = 0; i < 8; ++i) v[i] = F::kLift != 0.0f ? ldexpf(v[i] * sign, up) : v[i] * sign;
       F::parts(v, q[c]);
     }
-    back = ldexpf(a.scale, -up);
+    back = ldexpf(fabsf(a.scale), -up);
   }
+  // Scores that are only scaled go into the exponential with one multiply-add.
+  const bool direct = score.plain && __all(back * kLog2e > 0.0f && back * kLog2e < INFINITY);
+  const float mul = direct ? back * kLog2e : 1.0f;
   f16v o[HC];
 #pragma unroll
   for (int d = 0; d < HC; ++d)
@@ -648,152 +667,132 @@ __global__ __launch_bounds__(256, HC <= 4 ? 2 : 1) void k_many(AttnArgs a, Layer
     for (int i = 0; i < 16; ++i) o[d][i] = 0.0f;
   float m = -INFINITY, l = 0.0f;
 
-  // Unit u of a stage's keys: 16 keys x 4 chunks of 8 dimensions per 64 units; of
-  // its values: 16 dimensions x 4 chunks of 8 keys.
-  Raw<T> raw[U];
-  auto key_unit = [](int u, int &key, int &chunk) {
-    key = (u & 15) + 16 * ((u >> 6) & 1);
-    chunk = ((u >> 4) & 3) + 4 * (u >> 7);
+  // What is never loaded (dimensions past the head, keys that are not there) is
+  // zero, or a value of an earlier stage.
+  for (int i = tid; i < 4 * BUF; i += 256) kl[i] = u4{0, 0, 0, 0};
+  const int kkey = row_key(col);
+  // Pages of the two halves of a stage: even and odd lanes look them up (the entry
+  // of the last position past the end), and each is a scalar only where it is used,
+  // a stage later: a scalar at once would wait for the DMA in flight.
+  auto entries = [&](int kb) { return table[min(kb + 16 * (lane & 1), hi - 1) >> kv.shift]; };
+  auto page_of_half = [&](int entry, int kb, int u) {
+    const int p = __builtin_amdgcn_readlane(entry, u);
+    return kb + 16 * u < hi && (unsigned)p < (unsigned)kv.pages ? p : -1;
   };
-  auto value_unit = [](int u, int &d, int &chunk) {
-    d = (u & 15) + 16 * (u >> 6);
-    chunk = (u >> 4) & 3;
-  };
-  auto mine = [&](int i) { return UNITS % 256 == 0 || tid + 256 * i < UNITS; };
-  auto load_keys = [&](int base) {
+  // This wave's operands of a stage: every fourth of the keys' (16 dimensions each)
+  // and of the values' (16 keys x 32 dimensions).
+  auto load = [&](int kb, const int (&page)[2], int buf) {
+    const int key = kb + kkey, kpage = kkey & 16 ? page[1] : page[0];
+    if (kpage >= 0 && key < hi && key >= seen) {
+      const T *p = kv.k + key_at(kpage, kvh, key & mask, kv.nkv, hd, kv.shift) + 8 * h;
 #pragma unroll
-    for (int i = 0; i < U; ++i) {
-      int key, chunk;
-      key_unit(tid + 256 * i, key, chunk);
-      key += base;
-      const int page = key < hi ? page_of(table, key, kv.shift, kv.pages) : -1;
-      if (page >= 0 && key >= seen && 8 * chunk < hd && mine(i))
-        raw[i].load(kv.k + key_at(page, kvh, key & mask, kv.nkv, hd, kv.shift) + 8 * chunk);
-      else
-        raw[i].zero();
+      for (int f = 0; f < KS; f += 4)
+        if (f + wave < KS && 16 * (f + wave) + 8 * h < hd) dma(p + 16 * (f + wave), kl + buf * BUF + (f + wave) * OP);
+    }
+#pragma unroll
+    for (int f = 0; f < KS; f += 4) {
+      const int u = (f + wave) / HC, d = 32 * ((f + wave) % HC) + col, vpage = u ? page[1] : page[0];
+      if (f + wave < KS && vpage >= 0 && d < hd)
+        dma(kv.v + value_at(vpage, kvh, (kb + 16 * u + 8 * h) & mask, kv.nkv, hd, kv.shift) + ((size_t)d << kv.shift),
+            vl + buf * BUF + (f + wave) * OP);
     }
   };
-  auto put_keys = [&](u4 *buf) {
-#pragma unroll
-    for (int i = 0; i < U; ++i) {
-      if (!mine(i)) break;
-      int key, chunk;
-      key_unit(tid + 256 * i, key, chunk);
-      u4 x[KP];
-      raw[i].parts(x);
-      u4 *to = buf + (chunk >> 1) * KP * 64 + (chunk & 1) * 32 + key_row(key);
-#pragma unroll
-      for (int j = 0; j < KP; ++j) to[j * 64] = x[j];
-    }
-  };
-  auto load_values = [&](int base) {
-#pragma unroll
-    for (int i = 0; i < U; ++i) {
-      int d, chunk;
-      value_unit(tid + 256 * i, d, chunk);
-      const int key = base + 8 * chunk;
-      const int page = key < hi ? page_of(table, key, kv.shift, kv.pages) : -1;
-      if (page >= 0 && d < hd && mine(i))
-        raw[i].load(kv.v + value_at(page, kvh, key & mask, kv.nkv, hd, kv.shift) + ((size_t)d << kv.shift));
-      else
-        raw[i].zero();
-    }
-  };
-  auto put_values = [&](u4 *buf, int base) {
-    const bool edge = base < seen || base + S > hi;
-#pragma unroll
-    for (int i = 0; i < U; ++i) {
-      if (!mine(i)) break;
-      int d, chunk;
-      value_unit(tid + 256 * i, d, chunk);
-      if (edge) raw[i].keep(seen - base - 8 * chunk, hi - base - 8 * chunk);
-      u4 x[KP];
-      raw[i].parts(x);
-      u4 *to = buf + ((chunk >> 1) * HC + (d >> 5)) * KP * 64 + (chunk & 1) * 32 + (d & 31);
-#pragma unroll
-      for (int j = 0; j < KP; ++j) to[j * 64] = x[j];
-    }
-  };
-
-  load_keys(lo);
-  put_keys(kl);
-  load_values(lo);
-  put_values(vl, lo);
+  int next = 0, page[2] = {-1, -1};
+  __syncthreads();
+  if (lo < hi) {
+    next = entries(lo);
+    page[0] = page_of_half(next, lo, 0);
+    page[1] = page_of_half(next, lo, 1);
+    next = entries(lo + S);
+    load(lo, page, 0);
+  }
   int cur = 0;
   for (int kb = lo; kb < hi; kb += S, cur ^= 1) {
-    const bool more = kb + S < hi, work = !idle && kb < whi && kb + S > wlo;
-    const u4 *kbuf = kl + cur * BUF, *vbuf = vl + (kValueBufs<T> > 1 ? cur : 0) * BUF;
+    const u4 *kbuf = kl + cur * BUF;
+    u4 *vbuf = vl + cur * BUF;
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
     __syncthreads();
-    if (more) load_keys(kb + S);
+    const bool now[2] = {page[0] >= 0, page[1] >= 0};
+    if (kb + S < hi) {
+      page[0] = page_of_half(next, kb + S, 0);
+      page[1] = page_of_half(next, kb + S, 1);
+      next = entries(kb + 2 * S);
+      load(kb + S, page, cur ^ 1);
+    }
+    const bool inside = kb >= seen && kb + S <= hi && now[0] && now[1];
+    if (!inside) {
+      // Slots that hold no key of these rows: whatever lies there becomes zero.
+      for (int f = wave; f < KS; f += 4) {
+        const int u = f / HC, vk = kb + 16 * u + 8 * h;
+        Raw<T> r;
+#pragma unroll
+        for (int i = 0; i < (int)sizeof(T) / 2; ++i) r.v[i] = vbuf[f * OP + lane + 64 * i];
+        r.keep(now[u] ? seen - vk : 8, hi - vk);
+#pragma unroll
+        for (int i = 0; i < (int)sizeof(T) / 2; ++i) vbuf[f * OP + lane + 64 * i] = r.v[i];
+      }
+      __syncthreads();
+    }
+    if (idle || kb >= whi || kb + S <= wlo) continue;
     f16v s;
-    if (work) {
 #pragma unroll
-      for (int i = 0; i < 16; ++i) s[i] = 0.0f;
+    for (int i = 0; i < 16; ++i) s[i] = 0.0f;
 #pragma unroll
-      for (int c = 0; c < KS; ++c) {
-        u4 x[KP];
-#pragma unroll
-        for (int j = 0; j < KP; ++j) x[j] = kbuf[(c * KP + j) * 64 + lane];
-        s = products<F>(x, q[c], s, [](u4 x, u4 y, f16v c) { return F::mma32(x, y, c); });
-      }
+    for (int c = 0; c < KS; ++c) {
+      u4 x[KP];
+      fetch<T>(kbuf + c * OP + lane, x);
+      s = products<F>(x, q[c], s, [](u4 x, u4 y, f16v c) { return F::mma32(x, y, c); });
     }
-    if (more) {
-      put_keys(kl + (cur ^ 1) * BUF);
-      load_values(kb + S);
+    // Register 8 u + j of a lane is key kb + 16 u + 8 h + j.
+    if (!direct) {
+      if (score.softcap > 0.0f)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) s[i] = score.softcap * cap_tanh(s[i] * back * score.inv_cap) * kLog2e;
+      else
+#pragma unroll
+        for (int i = 0; i < 16; ++i) s[i] *= back * kLog2e;
+      if (a.slopes)
+#pragma unroll
+        for (int i = 0; i < 16; ++i)
+          s[i] = fmaf(-score.slope * kLog2e, (float)(pos - (kb + 16 * (i / 8) + 8 * h + i % 8)), s[i]);
     }
-    if (work) {
-      // Register 8 u + j of a lane is key kb + 16 u + 8 h + j.
-      float x[16], top = -INFINITY;
-      bool whole = kb >= alo && kb + S <= ahi && kb + S <= hi;
-      // Pages that are not there: looked up again, a page (16 keys or more) per u.
-      bool there[2];
-#pragma unroll
-      for (int u = 0; u < 2; ++u) {
-        there[u] = kb + 16 * u < hi && page_of(table, kb + 16 * u, kv.shift, kv.pages) >= 0;
-        whole = whole && there[u];
-      }
-#pragma unroll
-      for (int i = 0; i < 16; ++i) x[i] = score(s[i] * back, pos - (kb + 16 * (i / 8) + 8 * h + i % 8));
-      if (!whole)
-#pragma unroll
-        for (int i = 0; i < 16; ++i) {
-          const int key = kb + 16 * (i / 8) + 8 * h + i % 8;
-          x[i] = there[i / 8] && key <= pos && key >= first && key < hi ? x[i] : -INFINITY;
-        }
-#pragma unroll
-      for (int i = 0; i < 16; ++i) top = fmaxf(top, x[i]);
-      top = fmaxf(top, __shfl_xor(top, 32));
-      const float mn = fmaxf(m, top), ref = (mn == -INFINITY ? 0.0f : mn) - F::kLift;
-      const float alpha = m == mn ? 1.0f : __builtin_amdgcn_exp2f(m - mn);
-      m = mn;
-      float sum = 0.0f;
+    if (!(inside && kb >= alo && kb + S <= ahi))
 #pragma unroll
       for (int i = 0; i < 16; ++i) {
-        x[i] = __builtin_amdgcn_exp2f(x[i] - ref);
-        sum += x[i];
+        const int key = kb + 16 * (i / 8) + 8 * h + i % 8;
+        s[i] = (now[i / 8] & (key <= pos) & (key >= first) & (key < hi)) ? s[i] : -INFINITY;
       }
-      l = l * alpha + sum;
-      if (__any(alpha != 1.0f))
+    float top = s[0];
 #pragma unroll
-        for (int d = 0; d < HC; ++d) o[d] *= alpha;
+    for (int i = 1; i < 16; ++i) top = fmaxf(top, s[i]);
+    top = fmaxf(top, __shfl_xor(top, 32));
+    const float mn = fmaxf(m, top * mul), ref = (mn == -INFINITY ? 0.0f : mn) - F::kLift;
+    const float alpha = m == mn ? 1.0f : __builtin_amdgcn_exp2f(m - mn);
+    m = mn;
+    float sum = 0.0f;
 #pragma unroll
-      for (int u = 0; u < 2; ++u) {
-        float y[8];
+    for (int i = 0; i < 16; ++i) {
+      s[i] = __builtin_amdgcn_exp2f(fmaf(s[i], mul, -ref));
+      sum += s[i];
+    }
+    l = l * alpha + sum;
+    if (__any(alpha != 1.0f))
 #pragma unroll
-        for (int j = 0; j < 8; ++j) y[j] = x[8 * u + j];
-        u4 p[P];
-        F::parts(y, p);
+      for (int d = 0; d < HC; ++d) o[d] *= alpha;
 #pragma unroll
-        for (int d = 0; d < HC; ++d) {
-          u4 v[KP];
+    for (int u = 0; u < 2; ++u) {
+      float y[8];
 #pragma unroll
-          for (int j = 0; j < KP; ++j) v[j] = vbuf[((u * HC + d) * KP + j) * 64 + lane];
-          o[d] = products<F>(v, p, o[d], [](u4 x, u4 y, f16v c) { return F::mma32(x, y, c); });
-        }
+      for (int j = 0; j < 8; ++j) y[j] = s[8 * u + j];
+      u4 p[P];
+      F::parts(y, p);
+#pragma unroll
+      for (int d = 0; d < HC; ++d) {
+        u4 v[KP];
+        fetch<T>(vbuf + (u * HC + d) * OP + lane, v);
+        o[d] = products<F>(v, p, o[d], [](u4 x, u4 y, f16v c) { return F::mma32(x, y, c); });
       }
     }
-    if (kValueBufs<T> == 1) __syncthreads();
-    if (more) put_values(vl + (kValueBufs<T> > 1 ? cur ^ 1 : 0) * BUF, kb + S);
   }
   l += __shfl_xor(l, 32);
   bool bad = !(fabsf(l) < INFINITY);
