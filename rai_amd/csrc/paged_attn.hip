@@ -53,16 +53,18 @@ __device__ __forceinline__ float wave_sum(float x) {
   return x;
 }
 
-// tanh: odd polynomial near zero (1 - 2 / (e^2x + 1) cancels there), error under
-// 2^-22 relative.
+// tanh.  Near zero, where 1 - 2 / (e^2x + 1) cancels, x + x^3 P(x^2) with P fitted to
+// the smallest relative error over 0..0.625 (4e-9).
+constexpr float kTanhNear = 0.625f;
+__device__ __forceinline__ float tanh_near(float x) {
+  const float y = x * x;
+  const float p = fmaf(fmaf(fmaf(fmaf(-0.005717044f, y, 0.020650586f), y, -0.053743497f), y, 0.13331491f), y, -0.33333284f);
+  return fmaf(x * y, p, x);
+}
 __device__ __forceinline__ float cap_tanh(float x) {
-  const float a = fabsf(x);
-  const float e = __builtin_amdgcn_exp2f(2.0f * kLog2e * a);
+  const float e = __builtin_amdgcn_exp2f(2.0f * kLog2e * fabsf(x));
   const float far = 1.0f - 2.0f * __builtin_amdgcn_rcpf(e + 1.0f);
-  const float y = a * a;
-  const float near =
-      a + a * y * (-0.33333333f + y * (0.13333333f + y * (-0.053968254f + y * (0.021869488f - y * 0.0088632355f))));
-  return copysignf(a < 0.4f ? near : far, x);
+  return fabsf(x) < kTanhNear ? tanh_near(x) : copysignf(far, x);
 }
 
 // A score in the log2 domain: x = q . k * scale.
@@ -83,8 +85,7 @@ __device__ __forceinline__ Score score_of(const AttnArgs &a, int head) {
 // ------------------------------------------------------------ rows and splits --
 
 // Rows of a sequence on one kv head: r = token * per + query head of the group.
-// Tile t holds rows t * R .. of them and reads positions lo .. hi - 1; a split is
-// `len` of those, from `lo` rounded down to a whole stage.
+// Tile t holds rows t * R .. of them and reads positions lo .. hi - 1.
 struct Tile {
   int lo, hi;  // lo: a multiple of 64
 };
@@ -92,7 +93,16 @@ __device__ __forceinline__ Tile tile_of(const SeqSpan &sp, int t, int R, int per
   const int base = sp.n - sp.nq, first = t * R / per, last = min(sp.nq - 1, (t * R + R - 1) / per);
   return {first_seen(base + first, window) & ~63, max(base + last + 1, 0)};
 }
-__device__ __forceinline__ int splits_of(const Tile &t, int len) { return t.hi > t.lo ? (t.hi - t.lo + len - 1) / len : 1; }
+// A tile's positions in equal splits of whole 128, as many as `len` asks for.
+struct Share {
+  int count, len;
+};
+__device__ __forceinline__ Share share_of(const Tile &t, int len) {
+  const int span = t.hi - t.lo;
+  if (span <= len) return {1, len};
+  const int n = (span + len - 1) / len, each = ((span + n - 1) / n + 127) & ~127;
+  return {(span + each - 1) / each, each};
+}
 
 constexpr int kFewRows = 16;    // a tile of k_few
 constexpr int kManyRows = 128;  // a tile of k_many
@@ -268,6 +278,11 @@ struct Raw {
 #pragma unroll
     for (int i = 0; i < (int)sizeof(T) / 2; ++i) v[i] = u4{0, 0, 0, 0};
   }
+  // A lane's values of an operand in LDS (f32: in two halves of 64 lanes).
+  __device__ __forceinline__ void fetch(const u4 *at) {
+#pragma unroll
+    for (int i = 0; i < (int)sizeof(T) / 2; ++i) v[i] = at[64 * i];
+  }
   // Keeps elements from .. to - 1 of the eight.
   __device__ __forceinline__ void keep(int from, int to) {
 #pragma unroll
@@ -290,15 +305,6 @@ struct Raw {
     }
   }
 };
-
-// A lane's eight values of an operand in LDS (f32: in two halves of 64 lanes).
-template <class T>
-__device__ __forceinline__ void fetch(const u4 *at, u4 (&x)[Form<T>::KP]) {
-  Raw<T> r;
-#pragma unroll
-  for (int i = 0; i < (int)sizeof(T) / 2; ++i) r.v[i] = at[64 * i];
-  r.parts(x);
-}
 
 // Values of a lane's keys in k_few: 16 bytes either way, eight of f16 or bf16, four
 // of f32.
@@ -358,9 +364,10 @@ __global__ __launch_bounds__(256) void k_few(AttnArgs a, LayerView<T> kv, BatchV
   const int rows = sp.nq * per;
   if (rows == 0 || !few_rows(sp.nq, per)) return;
   const Tile tile = tile_of(sp, 0, kFewRows, per, a.window);
-  const int splits = splits_of(tile, sl.few_len);
+  const Share each = share_of(tile, sl.few_len);
+  const int splits = each.count;
   if (split >= splits) return;
-  const int lo = tile.lo + split * sl.few_len, hi = min(tile.hi, lo + sl.few_len);
+  const int lo = tile.lo + split * each.len, hi = min(tile.hi, lo + each.len);
   const int seen = first_seen(sp.n - sp.nq, a.window);  // no row sees less
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, col = lane & 15, g = lane >> 4;
   const int *table = b.tables + (size_t)seq * b.stride;
@@ -582,7 +589,7 @@ constexpr int kStage = 32;
 
 template <class T, int HC>
 constexpr size_t many_lds() {
-  return (size_t)2 * 2 * kStage * HC * 32 * sizeof(T);
+  return (size_t)kStage * HC * 32 * 2 * (sizeof(T) == 4 ? 4 + 3 * 2 : 2 * 2);
 }
 
 typedef __attribute__((address_space(3))) void lds_void;
@@ -604,8 +611,11 @@ __global__ __launch_bounds__(256, HC <= 4 ? 2 : 1) void k_many(AttnArgs a, Layer
   using F = Form<T>;
   constexpr int KP = F::KP, P = F::P, S = kStage, KS = 2 * HC;
   constexpr int OP = 64 * sizeof(T) / 2, BUF = KS * OP;  // an operand, and a stage of keys or of values, in 16 bytes
+  constexpr bool CUT = KP > 1;
+  constexpr int BUFS = CUT ? 1 : 2, PART = 64 * KP;  // an operand in parts
   extern __shared__ __align__(16) uint8_t lds[];
-  u4 *kl = reinterpret_cast<u4 *>(lds), *vl = kl + 2 * BUF;
+  u4 *kl = reinterpret_cast<u4 *>(lds), *vl = kl + BUFS * BUF;
+  u4 *kparts = CUT ? vl + BUF : kl, *vparts = CUT ? kparts + KS * PART : vl;
   const int seq = blockIdx.z, split = blockIdx.y, per = a.heads / kv.nkv, hd = kv.hd;
   const SeqSpan sp = seq_span(b, seq);
   const int rows = sp.nq * per, tiles = (rows + kManyRows - 1) / kManyRows;
@@ -613,9 +623,10 @@ __global__ __launch_bounds__(256, HC <= 4 ? 2 : 1) void k_many(AttnArgs a, Layer
   const int kvh = blockIdx.x % kv.nkv, t = tiles - 1 - (int)(blockIdx.x / kv.nkv);
   if (t < 0 || few_rows(sp.nq, per)) return;
   const Tile tile = tile_of(sp, t, kManyRows, per, a.window);
-  const int splits = splits_of(tile, sl.many_len);
+  const Share each = share_of(tile, sl.many_len);
+  const int splits = each.count;
   if (split >= splits) return;
-  const int lo = tile.lo + split * sl.many_len, hi = min(tile.hi, lo + sl.many_len);
+  const int lo = tile.lo + split * each.len, hi = min(tile.hi, lo + each.len);
   const int base0 = sp.n - sp.nq;
   const int seen = first_seen(base0 + t * kManyRows / per, a.window);
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, col = lane & 31, h = lane >> 5;
@@ -669,7 +680,7 @@ __global__ __launch_bounds__(256, HC <= 4 ? 2 : 1) void k_many(AttnArgs a, Layer
 
   // What is never loaded (dimensions past the head, keys that are not there) is
   // zero, or a value of an earlier stage.
-  for (int i = tid; i < 4 * BUF; i += 256) kl[i] = u4{0, 0, 0, 0};
+  for (int i = tid; i < 2 * BUFS * BUF; i += 256) kl[i] = u4{0, 0, 0, 0};
   const int kkey = row_key(col);
   // Pages of the two halves of a stage: even and odd lanes look them up (the entry
   // of the last position past the end), and each is a scalar only where it is used,
@@ -707,32 +718,42 @@ __global__ __launch_bounds__(256, HC <= 4 ? 2 : 1) void k_many(AttnArgs a, Layer
     load(lo, page, 0);
   }
   int cur = 0;
-  for (int kb = lo; kb < hi; kb += S, cur ^= 1) {
-    const u4 *kbuf = kl + cur * BUF;
-    u4 *vbuf = vl + cur * BUF;
+  for (int kb = lo; kb < hi; kb += S, cur ^= BUFS - 1) {
+    const u4 *kbuf = kparts + cur * BUF;
+    u4 *vbuf = vparts + cur * BUF;
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
     __syncthreads();
-    const bool now[2] = {page[0] >= 0, page[1] >= 0};
-    if (kb + S < hi) {
+    const bool now[2] = {page[0] >= 0, page[1] >= 0}, inside = kb >= seen && kb + S <= hi && now[0] && now[1];
+    auto ahead = [&] {
+      if (kb + S >= hi) return;
       page[0] = page_of_half(next, kb + S, 0);
       page[1] = page_of_half(next, kb + S, 1);
       next = entries(kb + 2 * S);
-      load(kb + S, page, cur ^ 1);
-    }
-    const bool inside = kb >= seen && kb + S <= hi && now[0] && now[1];
-    if (!inside) {
+      load(kb + S, page, CUT ? 0 : cur ^ 1);
+    };
+    if (!CUT) ahead();
+    if (CUT || !inside) {
       // Slots that hold no key of these rows: whatever lies there becomes zero.
+#pragma unroll
       for (int f = wave; f < KS; f += 4) {
         const int u = f / HC, vk = kb + 16 * u + 8 * h;
         Raw<T> r;
+        u4 x[KP];
+        if constexpr (CUT) {
+          r.fetch(kl + f * OP + lane);
+          r.parts(x);
 #pragma unroll
-        for (int i = 0; i < (int)sizeof(T) / 2; ++i) r.v[i] = vbuf[f * OP + lane + 64 * i];
-        r.keep(now[u] ? seen - vk : 8, hi - vk);
+          for (int j = 0; j < KP; ++j) kparts[f * PART + 64 * j + lane] = x[j];
+        }
+        r.fetch((CUT ? vl : vbuf) + f * OP + lane);
+        if (!inside) r.keep(now[u] ? seen - vk : 8, hi - vk);
+        r.parts(x);
 #pragma unroll
-        for (int i = 0; i < (int)sizeof(T) / 2; ++i) vbuf[f * OP + lane + 64 * i] = r.v[i];
+        for (int j = 0; j < KP; ++j) vbuf[f * PART + 64 * j + lane] = x[j];
       }
       __syncthreads();
     }
+    if (CUT) ahead();
     if (idle || kb >= whi || kb + S <= wlo) continue;
     f16v s;
 #pragma unroll
@@ -740,17 +761,30 @@ __global__ __launch_bounds__(256, HC <= 4 ? 2 : 1) void k_many(AttnArgs a, Layer
 #pragma unroll
     for (int c = 0; c < KS; ++c) {
       u4 x[KP];
-      fetch<T>(kbuf + c * OP + lane, x);
+#pragma unroll
+      for (int j = 0; j < KP; ++j) x[j] = kbuf[c * PART + 64 * j + lane];
       s = products<F>(x, q[c], s, [](u4 x, u4 y, f16v c) { return F::mma32(x, y, c); });
     }
     // Register 8 u + j of a lane is key kb + 16 u + 8 h + j.
     if (!direct) {
-      if (score.softcap > 0.0f)
+      if (score.softcap > 0.0f) {
+        const float in = back * score.inv_cap, out = score.softcap * kLog2e;
+        float most = 0.0f;
 #pragma unroll
-        for (int i = 0; i < 16; ++i) s[i] = score.softcap * cap_tanh(s[i] * back * score.inv_cap) * kLog2e;
-      else
+        for (int i = 0; i < 16; ++i) {
+          s[i] *= in;
+          most = fmaxf(most, fabsf(s[i]));
+        }
+        if (__all(most < kTanhNear))
+#pragma unroll
+          for (int i = 0; i < 16; ++i) s[i] = out * tanh_near(s[i]);
+        else
+#pragma unroll
+          for (int i = 0; i < 16; ++i) s[i] = out * cap_tanh(s[i]);
+      } else {
 #pragma unroll
         for (int i = 0; i < 16; ++i) s[i] *= back * kLog2e;
+      }
       if (a.slopes)
 #pragma unroll
         for (int i = 0; i < 16; ++i)
@@ -789,7 +823,8 @@ __global__ __launch_bounds__(256, HC <= 4 ? 2 : 1) void k_many(AttnArgs a, Layer
 #pragma unroll
       for (int d = 0; d < HC; ++d) {
         u4 v[KP];
-        fetch<T>(vbuf + (u * HC + d) * OP + lane, v);
+#pragma unroll
+        for (int j = 0; j < KP; ++j) v[j] = vbuf[(u * HC + d) * PART + 64 * j + lane];
         o[d] = products<F>(v, p, o[d], [](u4 x, u4 y, f16v c) { return F::mma32(x, y, c); });
       }
     }
@@ -845,7 +880,7 @@ __global__ __launch_bounds__(256) void k_join(AttnArgs a, BatchView b, Splits sl
   const int unit = blockIdx.x * (8 / shares) + w / shares, j = unit / a.heads, head = unit % a.heads, per = a.heads / nkv;
   const bool few = few_rows(sp.nq, per);
   const int R = few ? kFewRows : kManyRows, len = few ? sl.few_len : sl.many_len;
-  const int splits = j < sp.nq ? splits_of(tile_of(sp, (j * per + head % per) / R, R, per, a.window), len) : 0;
+  const int splits = j < sp.nq ? share_of(tile_of(sp, (j * per + head % per) / R, R, per, a.window), len).count : 0;
   const size_t at = part_at(a, b, 0, sp.q0 + min(j, max(sp.nq - 1, 0)), head), step = (size_t)b.tokens * a.heads;
   f4 o[2] = {f4{0, 0, 0, 0}, f4{0, 0, 0, 0}};
   float l = 0.0f;
