@@ -198,16 +198,6 @@ __global__ __launch_bounds__(kThreads) void k_beam_chunk(BeamArgs a, Parts out, 
   for (int i = n + tid; i < a.take; i += kThreads) keys[i * lists] = 0;
 }
 
-// n / d for n < 2^31: the high half of n times ceil(2^(32 + s) / d) - 2^32, plus n.
-struct Div {
-  uint32_t d, m, s;
-  explicit Div(uint32_t by) : d(by), s(0) {
-    while ((uint64_t(1) << s) < by) ++s;
-    m = (uint32_t)(((uint64_t(1) << 32) * ((uint64_t(1) << s) - by)) / by + 1);
-  }
-  __device__ __forceinline__ uint32_t operator()(uint32_t n) const { return (__umulhi(m, n) + n) >> s; }
-};
-
 constexpr int kBatch = 2048;  // candidates looked at in one go
 
 // One block per group: the chunks' lists merged, their first places first.  A

@@ -51,6 +51,16 @@ __device__ __forceinline__ Bf16 from_f32<Bf16>(float x) {
   return Bf16{(uint16_t)((u + 0x7fffu + ((u >> 16) & 1)) >> 16)};
 }
 
+// n / d for n < 2^31: the high half of n times ceil(2^(32 + s) / d) - 2^32, plus n.
+struct Div {
+  uint32_t d, m, s;
+  explicit Div(uint32_t by) : d(by), s(0) {
+    while ((uint64_t(1) << s) < by) ++s;
+    m = (uint32_t)(((uint64_t(1) << 32) * ((uint64_t(1) << s) - by)) / by + 1);
+  }
+  __device__ __forceinline__ uint32_t operator()(uint32_t n) const { return (__umulhi(m, n) + n) >> s; }
+};
+
 struct AttnArgs {
   const float *q;
   float *out;

@@ -49,59 +49,147 @@ __device__ __forceinline__ void pair_of(const RopeView &r, int i, int &e0, int &
   e1 = r.inter ? 2 * i + 1 : i + r.rot / 2;
 }
 
-// A block per row: queries and keys pair by pair, values element by element.
+constexpr int kTokens = 32;   // positions of a block, from a multiple of it on
+constexpr int kValueDims = 64;  // value elements of a block
+
+// Four elements as they go to the cache.
 template <class T>
-__global__ __launch_bounds__(256) void k_store(StoreArgs a, LayerView<T> kv, BatchView b) {
-  const SeqSpan sp = seq_span(b, blockIdx.y);
-  const int j = blockIdx.x;
-  if (j >= sp.nq) return;
-  __shared__ float cs[kMaxHd / 2], sn[kMaxHd / 2];
-  const int row = sp.q0 + j, pos = sp.n - sp.nq + j, half = a.rope.rot / 2;
-  for (int i = threadIdx.x; i < half; i += 256) rope_angle(pos, a.rope.inv[i], a.rope.gain, cs[i], sn[i]);
+__device__ __forceinline__ void put4(T *o, const float (&x)[4]) {
+  T y[4] = {from_f32<T>(x[0]), from_f32<T>(x[1]), from_f32<T>(x[2]), from_f32<T>(x[3])};
+  if constexpr (sizeof(T) == 4)
+    *reinterpret_cast<uint4 *>(o) = __builtin_bit_cast(uint4, y);
+  else
+    *reinterpret_cast<uint2 *>(o) = __builtin_bit_cast(uint2, y);
+}
+
+__device__ __forceinline__ void get4(const float *p, float (&x)[4]) {
+  const float4 v = *reinterpret_cast<const float4 *>(p);
+  x[0] = v.x, x[1] = v.y, x[2] = v.z, x[3] = v.w;
+}
+
+// Block (32 positions, part, sequence).  Parts below qk rotate a few heads of the
+// queries and keys, the angles of their positions computed once; the others take 64
+// elements of the values' rows: a thread has one element of eight positions, which
+// lie side by side in the page.  Bound by memory: 4 or 8 elements at a time (VEC: rows
+// 16-byte aligned, pairs in whole fours), each line of the pages written by one block.
+template <class T, bool VEC>
+__global__ __launch_bounds__(256) void k_store(StoreArgs a, LayerView<T> kv, BatchView b, int qk, int heads, Div by_units) {
+  __shared__ __align__(16) float cs[kTokens][kMaxHd / 2], sn[kTokens][kMaxHd / 2];
+  __shared__ int pages[kTokens];
+  const SeqSpan sp = seq_span(b, blockIdx.z);
+  const int base = sp.n - sp.nq, p0 = ((base >> 5) + (int)blockIdx.x) * kTokens, tid = threadIdx.x, hd = kv.hd;
+  const int j0 = max(p0 - base, 0), j1 = min(sp.nq, p0 + kTokens - base);
+  if (j0 >= j1) return;
+  const int *table = b.tables + (size_t)blockIdx.z * b.stride;
+  const int mask = (1 << kv.shift) - 1, part = blockIdx.y;
+  if (part >= qk) {
+    const int e = (part - qk) * kValueDims + (tid & 63), p = p0 + 8 * (tid >> 6);
+    if (e >= kv.nkv * hd || p + 8 <= base + j0 || p >= base + j1 || p + 7 < 0) return;
+    // Eight positions from a multiple of eight on share a page.
+    const int page = page_of(table, max(p, 0), kv.shift, kv.pages);
+    if (page < 0) return;
+    float x[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const int j = p + i - base;
+      x[i] = j >= j0 && j < j1 ? a.v[(size_t)(sp.q0 + j) * a.v_ld + e] : 0.0f;
+    }
+    T *o = kv.v + value_at(page, e / hd, p & mask, kv.nkv, hd, kv.shift) + ((size_t)(e % hd) << kv.shift);
+    if (p >= base + j0 && p + 8 <= base + j1 && p >= 0) {
+      put4(o, {x[0], x[1], x[2], x[3]});
+      put4(o + 4, {x[4], x[5], x[6], x[7]});
+    } else {
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+        if (p + i >= max(base + j0, 0) && p + i < base + j1) o[i] = from_f32<T>(x[i]);
+    }
+    return;
+  }
+  const int half = a.rope.rot / 2, rows = j1 - j0;
+  for (int i = tid; i < rows * half; i += 256) {
+    const int t = i / half, f = i - t * half;
+    rope_angle(base + j0 + t, a.rope.inv[f], a.rope.gain, cs[t][f], sn[t][f]);
+  }
+  for (int t = tid; t < rows; t += 256)
+    pages[t] = base + j0 + t >= 0 ? page_of(table, base + j0 + t, kv.shift, kv.pages) : -1;
   __syncthreads();
-  const int hd = kv.hd, units = half + (hd - a.rope.rot);  // of a head: pairs, then single elements
-  for (int u = threadIdx.x; u < a.heads * units; u += 256) {
-    const int h = u / units, i = u % units;
-    const float *x = a.q + (size_t)row * a.q_ld + (size_t)h * hd;
-    float *o = a.q_out + (size_t)row * a.qo_ld + (size_t)h * hd;
-    if (i < half) {
-      int e0, e1;
-      pair_of(a.rope, i, e0, e1);
-      const float x0 = x[e0], x1 = x[e1];
-      o[e0] = x0 * cs[i] - x1 * sn[i];
-      o[e1] = x1 * cs[i] + x0 * sn[i];
+  // Units of a row of a head: fours of pairs, then fours of other elements; or, one
+  // by one, pairs, then elements.
+  const int h0 = part * heads, h1 = min(h0 + heads, a.heads + kv.nkv), units = by_units.d;
+  const int pairs = VEC ? (a.rope.inter ? a.rope.rot / 4 : a.rope.rot / 8) : half;
+  for (int i = tid; i < (h1 - h0) * rows * units; i += 256) {
+    const int r = by_units(i), u = i - r * units, t = r % rows, h = h0 + r / rows;
+    const bool key = h >= a.heads;
+    const int page = pages[t];
+    if (key && page < 0) continue;
+    const size_t row = sp.q0 + j0 + t;
+    const float *x = key ? a.k + row * a.k_ld + (size_t)(h - a.heads) * hd : a.q + row * a.q_ld + (size_t)h * hd;
+    float *qo = a.q_out + row * a.qo_ld + (size_t)h * hd;
+    T *ko = kv.k + key_at(max(page, 0), key ? h - a.heads : 0, (base + j0 + t) & mask, kv.nkv, hd, kv.shift);
+    if constexpr (VEC) {
+      auto out = [&](int e, const float (&y)[4]) {
+        if (key)
+          put4(ko + e, y);
+        else
+          *reinterpret_cast<float4 *>(qo + e) = make_float4(y[0], y[1], y[2], y[3]);
+      };
+      float y[4], z[4];
+      if (u >= pairs) {
+        const int e = a.rope.rot + 4 * (u - pairs);
+        get4(x + e, y);
+        out(e, y);
+      } else if (a.rope.inter) {
+        get4(x + 4 * u, y);
+        const float c0 = cs[t][2 * u], s0 = sn[t][2 * u], c1 = cs[t][2 * u + 1], s1 = sn[t][2 * u + 1];
+        out(4 * u, {y[0] * c0 - y[1] * s0, y[1] * c0 + y[0] * s0, y[2] * c1 - y[3] * s1, y[3] * c1 + y[2] * s1});
+      } else {
+        get4(x + 4 * u, y);
+        get4(x + half + 4 * u, z);
+        float c[4], s[4];
+        get4(&cs[t][4 * u], c);
+        get4(&sn[t][4 * u], s);
+        out(4 * u, {y[0] * c[0] - z[0] * s[0], y[1] * c[1] - z[1] * s[1], y[2] * c[2] - z[2] * s[2], y[3] * c[3] - z[3] * s[3]});
+        out(half + 4 * u,
+            {z[0] * c[0] + y[0] * s[0], z[1] * c[1] + y[1] * s[1], z[2] * c[2] + y[2] * s[2], z[3] * c[3] + y[3] * s[3]});
+      }
     } else {
-      o[a.rope.rot + i - half] = x[a.rope.rot + i - half];
+      auto out = [&](int e, float y) {
+        if (key)
+          ko[e] = from_f32<T>(y);
+        else
+          qo[e] = y;
+      };
+      if (u < pairs) {
+        int e0, e1;
+        pair_of(a.rope, u, e0, e1);
+        const float x0 = x[e0], x1 = x[e1];
+        out(e0, x0 * cs[t][u] - x1 * sn[t][u]);
+        out(e1, x1 * cs[t][u] + x0 * sn[t][u]);
+      } else {
+        out(a.rope.rot + u - pairs, x[a.rope.rot + u - pairs]);
+      }
     }
-  }
-  if (pos < 0) return;
-  const int page = page_of(b.tables + (size_t)blockIdx.y * b.stride, pos, kv.shift, kv.pages);
-  if (page < 0) return;
-  const int slot = pos & ((1 << kv.shift) - 1);
-  for (int u = threadIdx.x; u < kv.nkv * units; u += 256) {
-    const int h = u / units, i = u % units;
-    const float *x = a.k + (size_t)row * a.k_ld + (size_t)h * hd;
-    T *o = kv.k + key_at(page, h, slot, kv.nkv, hd, kv.shift);
-    if (i < half) {
-      int e0, e1;
-      pair_of(a.rope, i, e0, e1);
-      const float x0 = x[e0], x1 = x[e1];
-      o[e0] = from_f32<T>(x0 * cs[i] - x1 * sn[i]);
-      o[e1] = from_f32<T>(x1 * cs[i] + x0 * sn[i]);
-    } else {
-      o[a.rope.rot + i - half] = from_f32<T>(x[a.rope.rot + i - half]);
-    }
-  }
-  for (int u = threadIdx.x; u < kv.nkv * hd; u += 256) {
-    const int h = u / hd, d = u % hd;
-    kv.v[value_at(page, h, slot, kv.nkv, hd, kv.shift) + ((size_t)d << kv.shift)] =
-        from_f32<T>(a.v[(size_t)row * a.v_ld + u]);
   }
 }
 
 template <class T>
 void launch_store(const StoreArgs &a, const LayerView<T> &kv, const BatchView &b, hipStream_t s) {
-  k_store<T><<<dim3(b.max_q, b.seqs), 256, 0, s>>>(a, kv, b);
+  const int rot = a.rope.rot, hd = kv.hd;
+  const uintptr_t all = (uintptr_t)a.q | (uintptr_t)a.q_out | (uintptr_t)a.k;
+  const bool vec = all % 16 == 0 && (a.q_ld | a.qo_ld | a.k_ld) % 4 == 0 && rot % (a.rope.inter ? 4 : 8) == 0;
+  const int pairs = vec ? rot / (a.rope.inter ? 4 : 8) : rot / 2, units = pairs + (vec ? (hd - rot) / 4 : hd - rot);
+  // Five heads a block where the batch is large (the angles are then a tenth of its
+  // work), fewer where blocks are few.
+  const int tiles = (b.max_q + kTokens - 2) / kTokens + 1, all_heads = a.heads + kv.nkv;
+  const size_t blocks = (size_t)tiles * b.seqs;
+  int heads = 5;
+  while (heads > 1 && blocks * ((all_heads + heads - 1) / heads) < 512) --heads;
+  const int qk = (all_heads + heads - 1) / heads, parts = qk + (kv.nkv * hd + kValueDims - 1) / kValueDims;
+  const dim3 grid(tiles, parts, b.seqs);
+  if (vec)
+    k_store<T, true><<<grid, 256, 0, s>>>(a, kv, b, qk, heads, Div(units));
+  else
+    k_store<T, false><<<grid, 256, 0, s>>>(a, kv, b, qk, heads, Div(units));
 }
 
 // ----------------------------------------------------------- forks and moves --
@@ -114,33 +202,37 @@ struct PoolBytes {
   int layers, pages;
 };
 
-__device__ __forceinline__ void copy_page(const PoolBytes &p, int layer, int src, int dst, int tid, int n) {
-  const size_t base = (size_t)layer * p.layer_vecs;
+// Keys and values of a page are copied by `parts` blocks, 32 KB of each at most.
+constexpr size_t kCopyVecs = 2048;
+
+__device__ __forceinline__ void copy_page(const PoolBytes &p, int layer, int src, int dst, int part) {
+  const size_t base = (size_t)layer * p.layer_vecs, from = part * kCopyVecs;
+  const size_t to = min(p.page_vecs, from + kCopyVecs);
   const uint4 *ks = p.k + base + (size_t)src * p.page_vecs, *vs = p.v + base + (size_t)src * p.page_vecs;
   uint4 *kd = p.k + base + (size_t)dst * p.page_vecs, *vd = p.v + base + (size_t)dst * p.page_vecs;
-  for (size_t i = tid; i < p.page_vecs; i += n) {
+#pragma unroll 4
+  for (size_t i = from + threadIdx.x; i < to; i += 256) {
     const uint4 x = ks[i], y = vs[i];
     kd[i] = x;
     vd[i] = y;
   }
 }
 
-// Block (layer, child): layer 0's blocks write the table row too.
+// Block (layer x part, child): the first one's blocks write the table row too.
 __global__ __launch_bounds__(256) void k_fork(PoolBytes p, const int *tables, size_t stride, const int *lengths,
-                                              int seqs, const int *parent, const int *fresh, int n, int *tables_out,
+                                              int seqs, const int *parent, const int *fresh, int parts, int *tables_out,
                                               int *lengths_out, int *used, int shift) {
   const int i = blockIdx.y, par = parent[i], tid = threadIdx.x;
   const bool ok = (unsigned)par < (unsigned)seqs;
   const size_t most = stride << shift;
-  int len = ok ? max(lengths[par], 0) : 0;
+  int len = ok ? max(lengths[par], 0) : 0, f = fresh[i];
   if ((size_t)len > most) len = (int)most;
   int again = 0;
   for (int j = tid; j < i; j += 256) again |= parent[j] == par;
   again = __syncthreads_or(again);
   const bool part = (len & ((1 << shift) - 1)) != 0, take = ok && part && again;
   const int last = len >> shift;  // the part-filled page's place
-  int f = take ? fresh[i] : -1;
-  if ((unsigned)f >= (unsigned)p.pages) f = -1;
+  if (!take || (unsigned)f >= (unsigned)p.pages) f = -1;
   if (blockIdx.x == 0) {
     for (size_t c = tid; c < stride; c += 256) {
       int id = ok ? tables[(size_t)par * stride + c] : -1;
@@ -152,27 +244,43 @@ __global__ __launch_bounds__(256) void k_fork(PoolBytes p, const int *tables, si
       used[i] = take && f >= 0;
     }
   }
-  if (!take || f < 0) return;
+  if (f < 0) return;
   const int src = tables[(size_t)par * stride + last];
   if ((unsigned)src >= (unsigned)p.pages) return;
-  copy_page(p, blockIdx.x, src, f, tid, 256);
+  copy_page(p, blockIdx.x / parts, src, f, blockIdx.x % parts);
 }
 
-__global__ __launch_bounds__(256) void k_move(PoolBytes p, const int *src, const int *dst, int n) {
-  const int a = src[blockIdx.y], b = dst[blockIdx.y];
-  if ((unsigned)a >= (unsigned)p.pages || (unsigned)b >= (unsigned)p.pages) return;
-  copy_page(p, blockIdx.x, a, b, threadIdx.x, 256);
-}
+constexpr int kRename = 2048;  // pairs looked through in one go
 
-__global__ __launch_bounds__(256) void k_rename(const int *src, const int *dst, int n, int pages, int *tables,
-                                                size_t entries) {
-  for (size_t e = (size_t)blockIdx.x * 256 + threadIdx.x; e < entries; e += (size_t)gridDim.x * 256) {
-    const int id = tables[e];
-    for (int i = 0; i < n; ++i)
-      if (src[i] == id && (unsigned)id < (unsigned)pages && (unsigned)dst[i] < (unsigned)pages) {
-        tables[e] = dst[i];
-        break;
+// Blocks 0 .. renames - 1: table entries, one a thread; the others: (pair, layer x part).
+__global__ __launch_bounds__(256) void k_move(PoolBytes p, const int *src, const int *dst, int n, int parts, int *tables,
+                                              size_t entries, int renames) {
+  __shared__ __align__(16) int from[kRename];
+  const int tid = threadIdx.x;
+  if ((int)blockIdx.x >= renames) {
+    const int copies = p.layers * parts, i = (blockIdx.x - renames) / copies, c = (blockIdx.x - renames) % copies;
+    const int a = src[i], b = dst[i];
+    if ((unsigned)a < (unsigned)p.pages && (unsigned)b < (unsigned)p.pages) copy_page(p, c / parts, a, b, c % parts);
+    return;
+  }
+  for (size_t e0 = (size_t)blockIdx.x * 256; e0 < entries; e0 += (size_t)renames * 256) {
+    const size_t e = e0 + tid;
+    const int id = e < entries ? tables[e] : -1;
+    int at = -1;
+    for (int i0 = 0; i0 < n; i0 += kRename) {
+      const int m = min(kRename, n - i0), m4 = (m + 3) & ~3;
+      __syncthreads();
+      for (int i = tid; i < m4; i += 256) from[i] = i < m ? src[i0 + i] : -1;
+      __syncthreads();
+#pragma unroll 4
+      for (int i = 0; i < m4; i += 4) {
+        const int4 f = *reinterpret_cast<const int4 *>(from + i);
+        at = f.x == id ? i0 + i : f.y == id ? i0 + i + 1 : f.z == id ? i0 + i + 2 : f.w == id ? i0 + i + 3 : at;
       }
+    }
+    if ((unsigned)id >= (unsigned)p.pages || at < 0) continue;
+    const int to = dst[at];
+    if ((unsigned)to < (unsigned)p.pages) tables[e] = to;
   }
 }
 
@@ -195,7 +303,7 @@ void check_pages(const rai_pages *p) {
   if (p->head_dim == 0 || p->head_dim % 8 || p->head_dim > kMaxHd)
     fail(RAI_E_SHAPE, "head_dim must be a multiple of 8 up to 256");
   if (p->layers == 0 || p->pages == 0 || p->kv_heads == 0) fail(RAI_E_SHAPE, "the pool must not be empty");
-  if (p->layers > 65535 || p->pages > INT32_MAX || p->kv_heads > 65535) fail(RAI_E_SHAPE, "dimensions overflow");
+  if (p->layers > 65535 || p->pages > INT32_MAX || p->kv_heads > 4096) fail(RAI_E_SHAPE, "dimensions overflow");
   if ((uintptr_t)p->k % 16 || (uintptr_t)p->v % 16) fail(RAI_E_ARG, "the pages must be 16-byte aligned");
 }
 
@@ -243,7 +351,7 @@ void with_layer(const rai_pages *p, size_t layer, F f) {
 }
 
 void check_heads(size_t heads, const rai_pages *p) {
-  if (heads == 0 || heads % p->kv_heads || heads > 65535)
+  if (heads == 0 || heads % p->kv_heads || heads > 16384)
     fail(RAI_E_SHAPE, "heads must be a positive multiple of kv_heads");
 }
 
@@ -316,7 +424,7 @@ int rai_paged_store_dev(const rai_pages *pages, size_t layer, const rai_page_bat
       if (!std::isfinite(rope->gain)) rai::fail(RAI_E_ARG, "gain must be finite");
       r = rai::RopeView{rope->inv_freq, (int)rope->rot_dim, rope->interleaved != 0, rope->gain};
     }
-    if (heads > 65535) rai::fail(RAI_E_SHAPE, "dimensions overflow");
+    if (heads > 16384) rai::fail(RAI_E_SHAPE, "dimensions overflow");
     if (!work) return RAI_OK;
     if (heads) {
       rai::check_rows(q, q_stride, heads, pages->head_dim, "q");
@@ -385,9 +493,11 @@ int rai_paged_fork_dev(const rai_pages *pages, const int32_t *tables, size_t tab
       rai::fail(RAI_E_ARG, "tables_out overlaps tables");
     if (lengths_out < lengths + seqs && lengths < lengths_out + n) rai::fail(RAI_E_ARG, "lengths_out overlaps lengths");
     const rai::PoolBytes p = rai::pool_bytes(pages);
-    rai::k_fork<<<dim3(p.layers, n), 256, 0, (hipStream_t)stream>>>(p, tables, table_stride, lengths, (int)seqs, parent,
-                                                                    fresh, (int)n, tables_out, lengths_out, used,
-                                                                    rai::page_shift(pages->page_size));
+    const int parts = (int)((p.page_vecs + rai::kCopyVecs - 1) / rai::kCopyVecs);
+    if ((size_t)p.layers * parts > (size_t(1) << 23)) rai::fail(RAI_E_SHAPE, "dimensions overflow");
+    rai::k_fork<<<dim3(p.layers * parts, n), 256, 0, (hipStream_t)stream>>>(
+        p, tables, table_stride, lengths, (int)seqs, parent, fresh, parts, tables_out, lengths_out, used,
+        rai::page_shift(pages->page_size));
     RAI_HIP_CHECK(hipGetLastError());
   });
 }
@@ -400,11 +510,10 @@ int rai_paged_move_dev(const rai_pages *pages, const int32_t *src, const int32_t
     if (!src || !dst || (!tables && entries)) rai::fail(RAI_E_ARG, "null argument");
     if (n > 65535) rai::fail(RAI_E_SHAPE, "at most 65535 pages in one call");
     const rai::PoolBytes p = rai::pool_bytes(pages);
-    hipStream_t s = (hipStream_t)stream;
-    rai::k_move<<<dim3(p.layers, n), 256, 0, s>>>(p, src, dst, (int)n);
-    if (entries)
-      rai::k_rename<<<(int)std::min<size_t>(1024, (entries + 255) / 256), 256, 0, s>>>(src, dst, (int)n, p.pages,
-                                                                                      tables, entries);
+    const size_t parts = (p.page_vecs + rai::kCopyVecs - 1) / rai::kCopyVecs, renames = std::min<size_t>(256, (entries + 255) / 256);
+    if (n * p.layers * parts >= size_t(1) << 23) rai::fail(RAI_E_SHAPE, "too many pages x layers in one call");
+    rai::k_move<<<(unsigned)(renames + n * p.layers * parts), 256, 0, (hipStream_t)stream>>>(p, src, dst, (int)n, (int)parts,
+                                                                                        tables, entries, (int)renames);
     RAI_HIP_CHECK(hipGetLastError());
   });
 }

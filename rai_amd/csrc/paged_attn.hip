@@ -612,6 +612,7 @@ __global__ __launch_bounds__(256, HC <= 4 ? 2 : 1) void k_many(AttnArgs a, Layer
   constexpr int KP = F::KP, P = F::P, S = kStage, KS = 2 * HC;
   constexpr int OP = 64 * sizeof(T) / 2, BUF = KS * OP;  // an operand, and a stage of keys or of values, in 16 bytes
   constexpr bool CUT = KP > 1;
+  constexpr int kPair = CUT ? 2 : 4;
   constexpr int BUFS = CUT ? 1 : 2, PART = 64 * KP;  // an operand in parts
   extern __shared__ __align__(16) uint8_t lds[];
   u4 *kl = reinterpret_cast<u4 *>(lds), *vl = kl + BUFS * BUF;
@@ -820,12 +821,22 @@ __global__ __launch_bounds__(256, HC <= 4 ? 2 : 1) void k_many(AttnArgs a, Layer
       for (int j = 0; j < 8; ++j) y[j] = s[8 * u + j];
       u4 p[P];
       F::parts(y, p);
+      // Two dimension tiles at a time: their sums do not wait for each other.
 #pragma unroll
-      for (int d = 0; d < HC; ++d) {
-        u4 v[KP];
+      for (int d0 = 0; d0 < HC; d0 += kPair) {
+        u4 v[kPair][KP];
 #pragma unroll
-        for (int j = 0; j < KP; ++j) v[j] = vbuf[(u * HC + d) * PART + 64 * j + lane];
-        o[d] = products<F>(v, p, o[d], [](u4 x, u4 y, f16v c) { return F::mma32(x, y, c); });
+        for (int d = 0; d < kPair; ++d)
+          if (d0 + d < HC)
+#pragma unroll
+            for (int j = 0; j < KP; ++j) v[d][j] = vbuf[(u * HC + d0 + d) * PART + 64 * j + lane];
+#pragma unroll
+        for (int w = (KP + P - 2 < P - 1 ? KP + P - 2 : P - 1); w >= 0; --w)
+#pragma unroll
+          for (int i = 0; i < KP; ++i)
+#pragma unroll
+            for (int d = 0; d < kPair; ++d)
+              if (d0 + d < HC && w - i >= 0 && w - i < P) o[d0 + d] = F::mma32(v[d][i], p[w - i], o[d0 + d]);
       }
     }
   }
