@@ -11,7 +11,7 @@ namespace rai {
 
 namespace {
 
-constexpr int kMaxHd = 256;
+constexpr int kMaxHd = 256;  // the angles of 32 positions: 32 KB of LDS at most
 
 // ------------------------------------------------------------------- store --
 
@@ -74,7 +74,7 @@ __device__ __forceinline__ void get4(const float *p, float (&x)[4]) {
 // 16-byte aligned, pairs in whole fours), each line of the pages written by one block.
 template <class T, bool VEC>
 __global__ __launch_bounds__(256) void k_store(StoreArgs a, LayerView<T> kv, BatchView b, int qk, int heads, Div by_units) {
-  __shared__ __align__(16) float cs[kTokens][kMaxHd / 2], sn[kTokens][kMaxHd / 2];
+  extern __shared__ __align__(16) float angles[];  // cosines [position][pair], sines behind them
   __shared__ int pages[kTokens];
   const SeqSpan sp = seq_span(b, blockIdx.z);
   const int base = sp.n - sp.nq, p0 = ((base >> 5) + (int)blockIdx.x) * kTokens, tid = threadIdx.x, hd = kv.hd;
@@ -106,67 +106,95 @@ __global__ __launch_bounds__(256) void k_store(StoreArgs a, LayerView<T> kv, Bat
     return;
   }
   const int half = a.rope.rot / 2, rows = j1 - j0;
+  float *const cs = angles, *const sn = angles + kTokens * half;
   for (int i = tid; i < rows * half; i += 256) {
     const int t = i / half, f = i - t * half;
-    rope_angle(base + j0 + t, a.rope.inv[f], a.rope.gain, cs[t][f], sn[t][f]);
+    rope_angle(base + j0 + t, a.rope.inv[f], a.rope.gain, cs[t * half + f], sn[t * half + f]);
   }
   for (int t = tid; t < rows; t += 256)
     pages[t] = base + j0 + t >= 0 ? page_of(table, base + j0 + t, kv.shift, kv.pages) : -1;
   __syncthreads();
   // Units of a row of a head: fours of pairs, then fours of other elements; or, one
-  // by one, pairs, then elements.
+  // by one, pairs, then elements.  Four units a thread are read before they are
+  // written (the output may be the input: a unit writes what it alone reads).
   const int h0 = part * heads, h1 = min(h0 + heads, a.heads + kv.nkv), units = by_units.d;
   const int pairs = VEC ? (a.rope.inter ? a.rope.rot / 4 : a.rope.rot / 8) : half;
-  for (int i = tid; i < (h1 - h0) * rows * units; i += 256) {
-    const int r = by_units(i), u = i - r * units, t = r % rows, h = h0 + r / rows;
-    const bool key = h >= a.heads;
-    const int page = pages[t];
-    if (key && page < 0) continue;
-    const size_t row = sp.q0 + j0 + t;
-    const float *x = key ? a.k + row * a.k_ld + (size_t)(h - a.heads) * hd : a.q + row * a.q_ld + (size_t)h * hd;
-    float *qo = a.q_out + row * a.qo_ld + (size_t)h * hd;
-    T *ko = kv.k + key_at(max(page, 0), key ? h - a.heads : 0, (base + j0 + t) & mask, kv.nkv, hd, kv.shift);
-    if constexpr (VEC) {
-      auto out = [&](int e, const float (&y)[4]) {
-        if (key)
-          put4(ko + e, y);
-        else
-          *reinterpret_cast<float4 *>(qo + e) = make_float4(y[0], y[1], y[2], y[3]);
-      };
-      float y[4], z[4];
-      if (u >= pairs) {
-        const int e = a.rope.rot + 4 * (u - pairs);
-        get4(x + e, y);
-        out(e, y);
-      } else if (a.rope.inter) {
-        get4(x + 4 * u, y);
-        const float c0 = cs[t][2 * u], s0 = sn[t][2 * u], c1 = cs[t][2 * u + 1], s1 = sn[t][2 * u + 1];
-        out(4 * u, {y[0] * c0 - y[1] * s0, y[1] * c0 + y[0] * s0, y[2] * c1 - y[3] * s1, y[3] * c1 + y[2] * s1});
+  const int bits = 32 - __clz(rows - 1), total = ((h1 - h0) << bits) * units;  // clz(0) is 32
+  constexpr int N = VEC ? 4 : 1, B = 4;
+  for (int i0 = tid; i0 < total; i0 += 256 * B) {
+    float y[B][N], z[B][N];
+    int unit[B], tok[B], head[B];
+#pragma unroll
+    for (int k = 0; k < B; ++k) {
+      const int i = i0 + 256 * k, r = by_units(i), u = i - r * units, t = r & ((1 << bits) - 1), h = h0 + (r >> bits);
+      const bool key = h >= a.heads, in = i < total && t < rows && (!key || pages[t] >= 0);
+      unit[k] = in ? u : -1;
+      tok[k] = t;
+      head[k] = h;
+      if (!in) continue;
+      const size_t row = sp.q0 + j0 + t;
+      const float *x = key ? a.k + row * a.k_ld + (size_t)(h - a.heads) * hd : a.q + row * a.q_ld + (size_t)h * hd;
+      int e0 = u, e1 = half + u;
+      if (VEC && u >= pairs)
+        e0 = a.rope.rot + 4 * (u - pairs);
+      else if (VEC)
+        e0 = 4 * u, e1 = half + 4 * u;
+      else if (u >= pairs)
+        e0 = a.rope.rot + u - pairs;
+      else if (a.rope.inter)
+        e0 = 2 * u, e1 = 2 * u + 1;
+      if constexpr (VEC) {
+        get4(x + e0, y[k]);
+        if (u < pairs && !a.rope.inter) get4(x + e1, z[k]);
       } else {
-        get4(x + 4 * u, y);
-        get4(x + half + 4 * u, z);
-        float c[4], s[4];
-        get4(&cs[t][4 * u], c);
-        get4(&sn[t][4 * u], s);
-        out(4 * u, {y[0] * c[0] - z[0] * s[0], y[1] * c[1] - z[1] * s[1], y[2] * c[2] - z[2] * s[2], y[3] * c[3] - z[3] * s[3]});
-        out(half + 4 * u,
-            {z[0] * c[0] + y[0] * s[0], z[1] * c[1] + y[1] * s[1], z[2] * c[2] + y[2] * s[2], z[3] * c[3] + y[3] * s[3]});
+        y[k][0] = x[e0];
+        if (u < pairs) z[k][0] = x[e1];
       }
-    } else {
-      auto out = [&](int e, float y) {
-        if (key)
-          ko[e] = from_f32<T>(y);
-        else
-          qo[e] = y;
-      };
-      if (u < pairs) {
-        int e0, e1;
-        pair_of(a.rope, u, e0, e1);
-        const float x0 = x[e0], x1 = x[e1];
-        out(e0, x0 * cs[t][u] - x1 * sn[t][u]);
-        out(e1, x1 * cs[t][u] + x0 * sn[t][u]);
+    }
+#pragma unroll
+    for (int k = 0; k < B; ++k) {
+      const int u = unit[k], t = tok[k], h = head[k];
+      if (u < 0) continue;
+      const bool key = h >= a.heads;
+      const size_t row = sp.q0 + j0 + t;
+      float *qo = a.q_out + row * a.qo_ld + (size_t)h * hd;
+      T *ko = kv.k + key_at(max(pages[t], 0), key ? h - a.heads : 0, (base + j0 + t) & mask, kv.nkv, hd, kv.shift);
+      if constexpr (VEC) {
+        auto out = [&](int e, const float (&v)[4]) {
+          if (key)
+            put4(ko + e, v);
+          else
+            *reinterpret_cast<float4 *>(qo + e) = make_float4(v[0], v[1], v[2], v[3]);
+        };
+        const float(&p)[4] = y[k], (&q)[4] = z[k];
+        if (u >= pairs) {
+          out(a.rope.rot + 4 * (u - pairs), p);
+        } else if (a.rope.inter) {
+          const float c0 = cs[t * half + 2 * u], s0 = sn[t * half + 2 * u], c1 = cs[t * half + 2 * u + 1], s1 = sn[t * half + 2 * u + 1];
+          out(4 * u, {p[0] * c0 - p[1] * s0, p[1] * c0 + p[0] * s0, p[2] * c1 - p[3] * s1, p[3] * c1 + p[2] * s1});
+        } else {
+          float c[4], s[4];
+          get4(&cs[t * half + 4 * u], c);
+          get4(&sn[t * half + 4 * u], s);
+          out(4 * u, {p[0] * c[0] - q[0] * s[0], p[1] * c[1] - q[1] * s[1], p[2] * c[2] - q[2] * s[2], p[3] * c[3] - q[3] * s[3]});
+          out(half + 4 * u,
+              {q[0] * c[0] + p[0] * s[0], q[1] * c[1] + p[1] * s[1], q[2] * c[2] + p[2] * s[2], q[3] * c[3] + p[3] * s[3]});
+        }
       } else {
-        out(a.rope.rot + u - pairs, x[a.rope.rot + u - pairs]);
+        auto out = [&](int e, float v) {
+          if (key)
+            ko[e] = from_f32<T>(v);
+          else
+            qo[e] = v;
+        };
+        if (u < pairs) {
+          int e0, e1;
+          pair_of(a.rope, u, e0, e1);
+          out(e0, y[k][0] * cs[t * half + u] - z[k][0] * sn[t * half + u]);
+          out(e1, z[k][0] * cs[t * half + u] + y[k][0] * sn[t * half + u]);
+        } else {
+          out(a.rope.rot + u - pairs, y[k][0]);
+        }
       }
     }
   }
@@ -186,10 +214,11 @@ void launch_store(const StoreArgs &a, const LayerView<T> &kv, const BatchView &b
   while (heads > 1 && blocks * ((all_heads + heads - 1) / heads) < 512) --heads;
   const int qk = (all_heads + heads - 1) / heads, parts = qk + (kv.nkv * hd + kValueDims - 1) / kValueDims;
   const dim3 grid(tiles, parts, b.seqs);
+  const size_t lds = (size_t)kTokens * rot * sizeof(float);
   if (vec)
-    k_store<T, true><<<grid, 256, 0, s>>>(a, kv, b, qk, heads, Div(units));
+    k_store<T, true><<<grid, 256, lds, s>>>(a, kv, b, qk, heads, Div(units));
   else
-    k_store<T, false><<<grid, 256, 0, s>>>(a, kv, b, qk, heads, Div(units));
+    k_store<T, false><<<grid, 256, lds, s>>>(a, kv, b, qk, heads, Div(units));
 }
 
 // ----------------------------------------------------------- forks and moves --
