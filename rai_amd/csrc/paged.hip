@@ -30,17 +30,20 @@ struct StoreArgs {
   RopeView rope;
 };
 
-// cos and sin of pos * inv, both times gain: the product and its reduction to
-// -pi..pi in f64 (an f32 angle of a far position is off by more than the rotation
-// may be), the functions of the reduced angle in f32.
+// cos and sin of pos * inv, both times gain.  The angle and its reduction to a
+// quarter turn and f, -1/2..1/2 of one, in f64 (an f32 angle of a far position is
+// off by more than the rotation may be); sin and cos of f quarter turns as
+// polynomials in f^2 with the smallest relative error (3e-9 and 6e-11, so f32's own
+// rounding is what is left).
 __device__ __forceinline__ void rope_angle(int pos, double inv, float gain, float &c, float &s) {
-  const double a = (double)pos * inv;
-  const double n = rint(a * 0.15915494309189535);
-  double r = fma(-n, 6.283185307179586, a);
-  r = fma(-n, 2.4492935982947064e-16, r);
-  sincosf((float)r, &s, &c);
-  c *= gain;
-  s *= gain;
+  const double a = (double)pos * (inv * 0.63661977236758138);
+  const double n = rint(a);
+  const float f = (float)(a - n), z = f * f;
+  const int k = (int)(n - 4.0 * floor(n * 0.25));
+  const float sf = f * fmaf(fmaf(fmaf(-0.00460165786f, z, 0.079680033f), z, -0.64596349f), z, 1.57079637f);
+  const float cf = fmaf(fmaf(fmaf(fmaf(0.00090336299f, z, -0.0208599363f), z, 0.253669173f), z, -1.23370051f), z, 1.0f);
+  c = gain * (k & 1 ? sf : cf) * ((k + 1) & 2 ? -1.0f : 1.0f);
+  s = gain * (k & 1 ? cf : sf) * (k & 2 ? -1.0f : 1.0f);
 }
 
 // The pair (e0, e1) of rotated pair i.
@@ -73,7 +76,7 @@ __device__ __forceinline__ void get4(const float *p, float (&x)[4]) {
 // lie side by side in the page.  Bound by memory: 4 or 8 elements at a time (VEC: rows
 // 16-byte aligned, pairs in whole fours), each line of the pages written by one block.
 template <class T, bool VEC>
-__global__ __launch_bounds__(256) void k_store(StoreArgs a, LayerView<T> kv, BatchView b, int qk, int heads, Div by_units) {
+__global__ __launch_bounds__(256) void k_store(StoreArgs a, LayerView<T> kv, BatchView b, int qk, int heads, Div by_units, Div by_half) {
   extern __shared__ __align__(16) float angles[];  // cosines [position][pair], sines behind them
   __shared__ int pages[kTokens];
   const SeqSpan sp = seq_span(b, blockIdx.z);
@@ -108,7 +111,7 @@ __global__ __launch_bounds__(256) void k_store(StoreArgs a, LayerView<T> kv, Bat
   const int half = a.rope.rot / 2, rows = j1 - j0;
   float *const cs = angles, *const sn = angles + kTokens * half;
   for (int i = tid; i < rows * half; i += 256) {
-    const int t = i / half, f = i - t * half;
+    const int t = by_half(i), f = i - t * half;
     rope_angle(base + j0 + t, a.rope.inv[f], a.rope.gain, cs[t * half + f], sn[t * half + f]);
   }
   for (int t = tid; t < rows; t += 256)
@@ -206,19 +209,17 @@ void launch_store(const StoreArgs &a, const LayerView<T> &kv, const BatchView &b
   const uintptr_t all = (uintptr_t)a.q | (uintptr_t)a.q_out | (uintptr_t)a.k;
   const bool vec = all % 16 == 0 && (a.q_ld | a.qo_ld | a.k_ld) % 4 == 0 && rot % (a.rope.inter ? 4 : 8) == 0;
   const int pairs = vec ? rot / (a.rope.inter ? 4 : 8) : rot / 2, units = pairs + (vec ? (hd - rot) / 4 : hd - rot);
-  // Five heads a block where the batch is large (the angles are then a tenth of its
-  // work), fewer where blocks are few.
+  // Two heads a block: all blocks of a large batch are then on the chip at once, and
+  // each has few loads to wait for (2241 rows of 32 + 8 heads: 31 us, with five 38).
   const int tiles = (b.max_q + kTokens - 2) / kTokens + 1, all_heads = a.heads + kv.nkv;
-  const size_t blocks = (size_t)tiles * b.seqs;
-  int heads = 5;
-  while (heads > 1 && blocks * ((all_heads + heads - 1) / heads) < 512) --heads;
+  const int heads = (size_t)tiles * b.seqs * all_heads < 1024 ? 1 : 2;
   const int qk = (all_heads + heads - 1) / heads, parts = qk + (kv.nkv * hd + kValueDims - 1) / kValueDims;
   const dim3 grid(tiles, parts, b.seqs);
   const size_t lds = (size_t)kTokens * rot * sizeof(float);
   if (vec)
-    k_store<T, true><<<grid, 256, lds, s>>>(a, kv, b, qk, heads, Div(units));
+    k_store<T, true><<<grid, 256, lds, s>>>(a, kv, b, qk, heads, Div(units), Div(std::max(rot / 2, 1)));
   else
-    k_store<T, false><<<grid, 256, lds, s>>>(a, kv, b, qk, heads, Div(units));
+    k_store<T, false><<<grid, 256, lds, s>>>(a, kv, b, qk, heads, Div(units), Div(std::max(rot / 2, 1)));
 }
 
 // ----------------------------------------------------------- forks and moves --

@@ -110,17 +110,18 @@ constexpr int kManyRows = 128;  // a tile of k_many
 // Sequences of at most kFewRows rows a kv head go to k_few, others to k_many.
 __device__ __forceinline__ bool few_rows(int nq, int per) { return nq * per <= kFewRows; }
 
-// How the key axis is split, and where the parts of a row's softmax lie:
-// [split][token row][head] x (hd values), and maximum and sum behind them.
-struct Splits {
-  int few_len, many_len, most;
+// How the key axis is split, and where the parts of a row's softmax lie: [row][split]
+// x hd values, and maximum and sum.  k_few's rows are kFewRows to a (sequence, kv
+// head), k_many's the heads of the batch's rows.
+struct Parts {
+  int len, most;
   float *o;
   float2 *ml;
+  __device__ __forceinline__ size_t at(size_t row, int split) const { return row * most + split; }
 };
-
-__device__ __forceinline__ size_t part_at(const AttnArgs &a, const BatchView &b, int split, int row, int head) {
-  return ((size_t)split * b.tokens + row) * a.heads + head;
-}
+struct Splits {
+  Parts few, many;
+};
 
 // -------------------------------------------------------------------- one row --
 
@@ -167,20 +168,19 @@ __device__ __forceinline__ void wave_row(const AttnArgs &a, const LayerView<T> &
   }
 }
 
-// A row's result again, from its own keys of positions lo .. hi - 1 (of the split).
+// A row's result again, from its own keys of positions lo .. hi - 1; as part `at` of
+// `parts` where the row is split.
 template <class T>
-__device__ __forceinline__ void redo_row(const AttnArgs &a, const LayerView<T> &kv, const BatchView &b, const Splits &sl,
-                                      const int *table, int row, int head, int pos, int lo, int hi, int split,
-                                      int splits) {
+__device__ __forceinline__ void redo_row(const AttnArgs &a, const LayerView<T> &kv, const int *table, int row, int head,
+                                         int pos, int lo, int hi, const Parts &parts, size_t at, bool split) {
   const int lane = threadIdx.x & 63;
   float m, l, o[4];
   wave_row(a, kv, table, head, a.q + (size_t)row * a.q_stride + (size_t)head * kv.hd, pos,
            max(lo, first_seen(pos, a.window)), min(hi, pos + 1), m, l, o);
   float *out = a.out + (size_t)row * a.out_stride + (size_t)head * kv.hd;
-  if (splits > 1) {
-    const size_t at = part_at(a, b, split, row, head);
-    out = sl.o + at * kv.hd;
-    if (lane == 0) sl.ml[at] = make_float2(m, l);
+  if (split) {
+    out = parts.o + at * kv.hd;
+    if (lane == 0) parts.ml[at] = make_float2(m, l);
     l = 1.0f;
   }
 #pragma unroll
@@ -350,7 +350,7 @@ __device__ __forceinline__ bool finite4(f4 x) {
 // values go into the f32 instructions as they come (their rate is four times what
 // memory gives; cutting them costs more).
 template <class T, int HC>  // HC: head size in steps of 32, rounded up
-__global__ __launch_bounds__(256) void k_few(AttnArgs a, LayerView<T> kv, BatchView b, Splits sl, bool vec) {
+__global__ __launch_bounds__(256, HC <= 4 ? 3 : 1) void k_few(AttnArgs a, LayerView<T> kv, BatchView b, Splits sl, bool vec) {
   using F = Form<T>;
   constexpr int KP = F::KP, P = F::P, D = 2 * HC;
   constexpr bool kF32 = sizeof(T) == 4;
@@ -364,11 +364,12 @@ __global__ __launch_bounds__(256) void k_few(AttnArgs a, LayerView<T> kv, BatchV
   const int rows = sp.nq * per;
   if (rows == 0 || !few_rows(sp.nq, per)) return;
   const Tile tile = tile_of(sp, 0, kFewRows, per, a.window);
-  const Share each = share_of(tile, sl.few_len);
+  const Share each = share_of(tile, sl.few.len);
   const int splits = each.count;
   if (split >= splits) return;
   const int lo = tile.lo + split * each.len, hi = min(tile.hi, lo + each.len);
   const int seen = first_seen(sp.n - sp.nq, a.window);  // no row sees less
+  const size_t row0 = ((size_t)seq * kv.nkv + kvh) * kFewRows;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, col = lane & 15, g = lane >> 4;
   const int *table = b.tables + (size_t)seq * b.stride;
   const int mask = (1 << kv.shift) - 1;
@@ -376,14 +377,21 @@ __global__ __launch_bounds__(256) void k_few(AttnArgs a, LayerView<T> kv, BatchV
   const int r = min(col, rows - 1), tok = r / per, head = kvh * per + r % per, pos = sp.n - sp.nq + tok;
   const int first = first_seen(pos, a.window);
   const Score score = score_of(a, head);
-  float qf[kF32 ? HC : 1][8];
-  u4 q[kF32 ? 1 : HC][P];
+  // The rows' queries as operands, the same for every wave, lane after lane.
+  constexpr int QP = kF32 ? 2 : P;
+  __shared__ u4 ql[HC][QP][64];
   float back = a.scale;
   {
     const float *x = a.q + (size_t)(sp.q0 + tok) * a.q_stride + (size_t)head * hd;
     if constexpr (kF32) {
+      for (int c = wave; c < HC; c += 4) {
+        float v[8];
+        query8(x, 32 * c + 8 * g, hd, vec, v);
 #pragma unroll
-      for (int c = 0; c < HC; ++c) query8(x, 32 * c + 8 * g, hd, vec, qf[c]);
+        for (int j = 0; j < 2; ++j)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) ql[c][j][lane][i] = __float_as_uint(v[4 * j + i]);
+      }
     } else {
       float v[HC][8], most = 0.0f;
 #pragma unroll
@@ -400,11 +408,16 @@ __global__ __launch_bounds__(256) void k_few(AttnArgs a, LayerView<T> kv, BatchV
         if (up)
 #pragma unroll
           for (int i = 0; i < 8; ++i) v[c][i] = ldexpf(v[c][i], up);
-        F::parts(v[c], q[c]);
+        u4 q[P];
+        F::parts(v[c], q);
+        if (c % 4 == wave)
+#pragma unroll
+          for (int j = 0; j < P; ++j) ql[c][j][lane] = q[j];
       }
       back = ldexpf(a.scale, -up);
     }
   }
+  __syncthreads();
   f4 o[D];
 #pragma unroll
   for (int d = 0; d < D; ++d) o[d] = f4{0, 0, 0, 0};
@@ -445,26 +458,32 @@ __global__ __launch_bounds__(256) void k_few(AttnArgs a, LayerView<T> kv, BatchV
   load_keys(base + ko, page_at(base + ko));
   load_values(base + vo, vpage);
   for (; base < hi; base += ALL) {
+    asm volatile("" ::: "memory");  // the queries are read from LDS each time: registers are for what is in flight
     const int vk = base + vo;
     f4 s[TK];
 #pragma unroll
     for (int t = 0; t < TK; ++t) s[t] = f4{0, 0, 0, 0};
 #pragma unroll
-    for (int c = 0; c < HC; ++c)
+    for (int c = 0; c < HC; ++c) {
+      u4 q[QP];
+#pragma unroll
+      for (int j = 0; j < QP; ++j) q[j] = ql[c][j][lane];
       if constexpr (kF32) {
 #pragma unroll
         for (int e = 0; e < 8; ++e)
 #pragma unroll
           for (int t = 0; t < TK; ++t)
-            s[t] = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(kr[t][c].v[e / 4][e % 4]), qf[c][e], s[t], 0, 0, 0);
+            s[t] = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(kr[t][c].v[e / 4][e % 4]),
+                                                        __uint_as_float(q[e / 4][e % 4]), s[t], 0, 0, 0);
       } else {
 #pragma unroll
         for (int t = 0; t < TK; ++t) {
           u4 x[KP];
           kr[t][c].parts(x);
-          s[t] = products<F>(x, q[c], s[t], [](u4 x, u4 y, f4 c) { return F::mma16(x, y, c); });
+          s[t] = products<F>(x, q, s[t], [](u4 x, u4 y, f4 c) { return F::mma16(x, y, c); });
         }
       }
+    }
     if (base + ALL < hi) load_keys(base + ALL + ko, knext);  // while this step's softmax and values go on
     float x[N], top = -INFINITY;
 #pragma unroll
@@ -549,13 +568,13 @@ __global__ __launch_bounds__(256) void k_few(AttnArgs a, LayerView<T> kv, BatchV
     const uint64_t all = __ballot(bad);
     if (lane == 0) bad_rows = (uint32_t)(all | all >> 16 | all >> 32 | all >> 48) & 0xffffu;
     if (col < rows) {
-      const size_t at = part_at(a, b, split, sp.q0 + tok, head);
+      const size_t at = sl.few.at(row0 + col, split);
       float *out = a.out + (size_t)(sp.q0 + tok) * a.out_stride + (size_t)head * hd;
       float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
       bool wide = vec;
       if (splits > 1) {
-        out = sl.o + at * hd;
-        if (g == 0) sl.ml[at] = make_float2(top - kLift, sum);
+        out = sl.few.o + at * hd;
+        if (g == 0) sl.few.ml[at] = make_float2(top - kLift, sum);
         inv = 1.0f;
         wide = true;
       }
@@ -575,7 +594,8 @@ __global__ __launch_bounds__(256) void k_few(AttnArgs a, LayerView<T> kv, BatchV
   if (bad_rows == 0) return;
   for (int i = wave; i < rows; i += 4)
     if (bad_rows >> i & 1)
-      redo_row(a, kv, b, sl, table, sp.q0 + i / per, kvh * per + i % per, sp.n - sp.nq + i / per, lo, hi, split, splits);
+      redo_row(a, kv, table, sp.q0 + i / per, kvh * per + i % per, sp.n - sp.nq + i / per, lo, hi, sl.few,
+               sl.few.at(row0 + i, split), splits > 1);
 }
 
 // ------------------------------------------------------------------- many rows --
@@ -624,7 +644,7 @@ __global__ __launch_bounds__(256, HC <= 4 ? 2 : 1) void k_many(AttnArgs a, Layer
   const int kvh = blockIdx.x % kv.nkv, t = tiles - 1 - (int)(blockIdx.x / kv.nkv);
   if (t < 0 || few_rows(sp.nq, per)) return;
   const Tile tile = tile_of(sp, t, kManyRows, per, a.window);
-  const Share each = share_of(tile, sl.many_len);
+  const Share each = share_of(tile, sl.many.len);
   const int splits = each.count;
   if (split >= splits) return;
   const int lo = tile.lo + split * each.len, hi = min(tile.hi, lo + each.len);
@@ -847,13 +867,13 @@ __global__ __launch_bounds__(256, HC <= 4 ? 2 : 1) void k_many(AttnArgs a, Layer
 #pragma unroll
     for (int i = 0; i < 16; ++i) bad = bad || !(fabsf(o[d][i]) < INFINITY);
   if (r0 + col < rows) {
-    const size_t at = part_at(a, b, split, sp.q0 + tok, head);
+    const size_t at = sl.many.at((size_t)(sp.q0 + tok) * a.heads + head, split);
     float *out = a.out + (size_t)(sp.q0 + tok) * a.out_stride + (size_t)head * hd;
     float inv = l == 0.0f ? 0.0f : 1.0f / l;
     bool wide = vec;
     if (splits > 1) {
-      out = sl.o + at * hd;
-      if (h == 0) sl.ml[at] = make_float2(m - F::kLift, l);
+      out = sl.many.o + at * hd;
+      if (h == 0) sl.many.ml[at] = make_float2(m - F::kLift, l);
       inv = 1.0f;
       wide = true;
     }
@@ -873,42 +893,51 @@ __global__ __launch_bounds__(256, HC <= 4 ? 2 : 1) void k_many(AttnArgs a, Layer
   const uint64_t all = __ballot(bad);
   for (uint32_t rest = (uint32_t)(all | all >> 32); rest; rest &= rest - 1) {
     const int i = r0 + __builtin_ctz(rest);
+    const int row = sp.q0 + i / per, hq = kvh * per + i % per;
     if (i < rows)
-      redo_row(a, kv, b, sl, table, sp.q0 + i / per, kvh * per + i % per, base0 + i / per, lo, hi, split, splits);
+      redo_row(a, kv, table, row, hq, base0 + i / per, lo, hi, sl.many, sl.many.at((size_t)row * a.heads + hq, split),
+               splits > 1);
   }
 }
 
 // ------------------------------------------------------------------------ join --
 
 // Splits of a row joined: 32 lanes x 4 dimensions (twice over for heads past 128)
-// by `shares` (1 to 8, a power of two) that take the splits in turn; a block has 8 /
-// shares rows.  Block (rows, sequence).
-__global__ __launch_bounds__(256) void k_join(AttnArgs a, BatchView b, Splits sl, int nkv, int hd, int shares, bool vec) {
-  __shared__ float ls[8];
-  __shared__ f4 part[8][64];
+// by `shares` (1 to 16, a power of two) that take the splits in turn; a block has 16
+// / shares rows.  Block (rows, sequence).  Bound by the latency of its loads: all of
+// a share's maxima are read at once, and its parts eight at a time.
+constexpr int kShares = 16;
+__global__ __launch_bounds__(32 * kShares) void k_join(AttnArgs a, BatchView b, Splits sl, int nkv, int hd, int shares,
+                                                       bool vec) {
+  __shared__ float ls[kShares];
+  __shared__ f4 part[kShares][64];
   const SeqSpan sp = seq_span(b, blockIdx.y);
   const int lane = threadIdx.x & 31, w = threadIdx.x >> 5, share = w & (shares - 1);
-  const int unit = blockIdx.x * (8 / shares) + w / shares, j = unit / a.heads, head = unit % a.heads, per = a.heads / nkv;
-  const bool few = few_rows(sp.nq, per);
-  const int R = few ? kFewRows : kManyRows, len = few ? sl.few_len : sl.many_len;
-  const int splits = j < sp.nq ? share_of(tile_of(sp, (j * per + head % per) / R, R, per, a.window), len).count : 0;
-  const size_t at = part_at(a, b, 0, sp.q0 + min(j, max(sp.nq - 1, 0)), head), step = (size_t)b.tokens * a.heads;
+  const int unit = blockIdx.x * (kShares / shares) + w / shares, j = unit / a.heads, head = unit % a.heads;
+  const int per = a.heads / nkv, kvh = head / per, r = j * per + head % per;
+  const bool few = few_rows(sp.nq, per), mine = j < sp.nq;
+  const int R = few ? kFewRows : kManyRows;
+  const Parts &parts = few ? sl.few : sl.many;
+  const int splits = mine ? share_of(tile_of(sp, r / R, R, per, a.window), parts.len).count : 0;
+  const size_t row = few ? ((size_t)blockIdx.y * nkv + kvh) * kFewRows + r : (size_t)(sp.q0 + j) * a.heads + head;
   f4 o[2] = {f4{0, 0, 0, 0}, f4{0, 0, 0, 0}};
   float l = 0.0f;
   if (splits > 1) {
+    const float2 *ml = parts.ml + parts.at(row, 0);
+    const float *p = parts.o + parts.at(row, 0) * hd + 4 * lane;
     float top = -INFINITY;
-    for (int s = lane; s < splits; s += 32) top = fmaxf(top, sl.ml[at + s * step].x);
+#pragma unroll 4
+    for (int s = lane; s < splits; s += 32) top = fmaxf(top, ml[s].x);
 #pragma unroll
     for (int d = 16; d; d >>= 1) top = fmaxf(top, __shfl_xor(top, d));
-#pragma unroll 4
+#pragma unroll 8
     for (int s = share; s < splits; s += shares) {
-      const float2 x = sl.ml[at + s * step];
+      const float2 x = ml[s];
       const float weight = x.x == top ? 1.0f : __builtin_amdgcn_exp2f(x.x - top);
       l += weight * x.y;
-      const float *p = sl.o + (at + s * step) * hd;
 #pragma unroll
       for (int i = 0; i < 2; ++i)
-        if (4 * lane + 128 * i < hd) o[i] += *reinterpret_cast<const f4 *>(p + 4 * lane + 128 * i) * weight;
+        if (4 * lane + 128 * i < hd) o[i] += *reinterpret_cast<const f4 *>(p + (size_t)s * hd + 128 * i) * weight;
     }
   }
   if (shares > 1) {
@@ -917,6 +946,7 @@ __global__ __launch_bounds__(256) void k_join(AttnArgs a, BatchView b, Splits sl
     part[w][lane + 32] = o[1];
     __syncthreads();
     if (share) return;
+#pragma unroll 4
     for (int s = 1; s < shares; ++s) {
       l += ls[w + s];
       o[0] += part[w + s][lane];
@@ -956,29 +986,34 @@ int most_keys(const BatchView &b, int window) {
 
 struct Plan {
   int few_len, many_len, few, many;  // split lengths and counts
-  bool use_few, use_many;
+  size_t few_rows, many_rows;
+  bool use_many;
+  size_t few_parts() const { return few > 1 ? few * few_rows : 0; }
+  size_t many_parts() const { return many > 1 ? many * many_rows : 0; }
 };
 
 Plan plan_of(int nkv, int heads, int hd, const BatchView &b, int window, size_t work_bytes) {
   Plan p;
   const int per = heads / nkv, keys = most_keys(b, window);
-  const size_t row_bytes = (size_t)b.tokens * heads * (4 * (size_t)hd + 8);
-  const size_t fit = std::max<size_t>(1, work_bytes / row_bytes);
   const size_t tiles = ((size_t)b.max_q * per + kManyRows - 1) / kManyRows;
-  p.use_few = true;
-  p.use_many = (size_t)b.max_q * per > kFewRows;
-  p.few_len = split_len((size_t)b.seqs * nkv, keys, 2048);
-  p.many_len = split_len((size_t)b.seqs * nkv * tiles, keys, 512);
-  auto count = [&](int &len) {
+  size_t left = work_bytes / (4 * (size_t)hd + 8);  // parts that fit
+  auto count = [&](int &len, size_t rows) {
     int n = (keys + len - 1) / len;
+    const size_t fit = std::max<size_t>(1, left / rows);
     if ((size_t)n > fit) {
-      len = (int)(((keys + fit - 1) / fit + 127) / 128 * 128);
+      len = (int)((((size_t)keys + fit - 1) / fit + 127) / 128 * 128);
       n = (keys + len - 1) / len;
     }
+    if (n > 1) left -= n * rows;
     return n;
   };
-  p.few = count(p.few_len);
-  p.many = count(p.many_len);
+  p.use_many = (size_t)b.max_q * per > kFewRows;
+  p.few_rows = (size_t)b.seqs * nkv * kFewRows;
+  p.many_rows = (size_t)b.tokens * heads;
+  p.few_len = split_len((size_t)b.seqs * nkv, keys, 2048);
+  p.few = count(p.few_len, p.few_rows);
+  p.many_len = split_len((size_t)b.seqs * nkv * tiles, keys, 512);
+  p.many = p.use_many ? count(p.many_len, p.many_rows) : 1;
   return p;
 }
 
@@ -991,24 +1026,25 @@ void launch_of(const AttnArgs &a, const LayerView<T> &kv, const BatchView &b, co
     dynamic_lds<k_many<T, HC>>(lds);
     k_many<T, HC><<<dim3((unsigned)(tiles * kv.nkv), p.many, b.seqs), 256, lds, s>>>(a, kv, b, sl, vec);
   }
-  if (p.use_few) k_few<T, HC><<<dim3(p.few, kv.nkv, b.seqs), 256, 0, s>>>(a, kv, b, sl, vec);
+  k_few<T, HC><<<dim3(p.few, kv.nkv, b.seqs), 256, 0, s>>>(a, kv, b, sl, vec);
 }
 
 }  // namespace
 
 size_t paged_attention_work(int nkv, int heads, int hd, const BatchView &b, int window) {
   const Plan p = plan_of(nkv, heads, hd, b, window, SIZE_MAX);
-  const int most = std::max(p.few, p.use_many ? p.many : 1);
-  return most > 1 ? (size_t)most * b.tokens * heads * (4 * (size_t)hd + 8) : 0;
+  return (p.few_parts() + p.many_parts()) * (4 * (size_t)hd + 8);
 }
 
 template <class T>
 void launch_paged_attention(const AttnArgs &a, const LayerView<T> &kv, const BatchView &b, void *work,
                             size_t work_bytes, hipStream_t s) {
   const Plan p = plan_of(kv.nkv, a.heads, kv.hd, b, a.window, work_bytes);
-  const int most = std::max(p.few, p.use_many ? p.many : 1);
-  Splits sl{p.few_len, p.many_len, most, static_cast<float *>(work), nullptr};
-  sl.ml = reinterpret_cast<float2 *>(sl.o + (size_t)most * b.tokens * a.heads * kv.hd);
+  Splits sl;
+  sl.few = Parts{p.few_len, p.few, static_cast<float *>(work), nullptr};
+  sl.many = Parts{p.many_len, p.many, sl.few.o + p.few_parts() * kv.hd, nullptr};
+  sl.few.ml = reinterpret_cast<float2 *>(sl.many.o + p.many_parts() * kv.hd);
+  sl.many.ml = sl.few.ml + p.few_parts();
   const bool vec = ((uintptr_t)a.q | (uintptr_t)a.out) % 16 == 0 && a.q_stride % 4 == 0 && a.out_stride % 4 == 0;
   switch ((kv.hd + 31) / 32) {
     case 1: launch_of<T, 1>(a, kv, b, p, sl, vec, s); break;
@@ -1017,12 +1053,14 @@ void launch_paged_attention(const AttnArgs &a, const LayerView<T> &kv, const Bat
     case 4: launch_of<T, 4>(a, kv, b, p, sl, vec, s); break;
     default: launch_of<T, 8>(a, kv, b, p, sl, vec, s); break;
   }
-  if (most > 1) {
+  if (p.few > 1 || p.many > 1) {
+    // By what most rows have.
+    const int most = p.use_many ? p.many : p.few;
     int shares = 1;
-    while (shares < 8 && 4 * shares < most) shares *= 2;
-    const int rows = 8 / shares;
-    k_join<<<dim3((unsigned)((b.max_q * a.heads + rows - 1) / rows), b.seqs), 256, 0, s>>>(a, b, sl, kv.nkv, kv.hd, shares,
-                                                                                           vec);
+    while (shares < kShares && 4 * shares < most) shares *= 2;
+    const int rows = kShares / shares;
+    k_join<<<dim3((unsigned)((b.max_q * a.heads + rows - 1) / rows), b.seqs), 32 * kShares, 0, s>>>(a, b, sl, kv.nkv, kv.hd,
+                                                                                                   shares, vec);
   }
 }
 
