@@ -107,12 +107,11 @@ __device__ __forceinline__ Share share_of(const Tile &t, int len) {
 constexpr int kFewRows = 16;    // a tile of k_few
 constexpr int kManyRows = 128;  // a tile of k_many
 
-// Sequences of at most kFewRows rows a kv head go to k_few, others to k_many.
-__device__ __forceinline__ bool few_rows(int nq, int per) { return nq * per <= kFewRows; }
 
-// How the key axis is split, and where the parts of a row's softmax lie: [row][split]
-// x hd values, and maximum and sum.  k_few's rows are kFewRows to a (sequence, kv
-// head), k_many's the heads of the batch's rows.
+// Sequences of at most few_max rows a kv head go to k_few, others to k_many.  How
+// the key axis is split, and where the parts of a row's softmax lie: [row][split] x hd
+// values, and maximum and sum.  k_few's rows are 16 few_tiles to a (sequence, kv head),
+// k_many's the heads of the batch's rows.
 struct Parts {
   int len, most;
   float *o;
@@ -120,7 +119,12 @@ struct Parts {
   __device__ __forceinline__ size_t at(size_t row, int split) const { return row * most + split; }
 };
 struct Splits {
+  int few_max, few_tiles;
   Parts few, many;
+  __device__ __forceinline__ bool is_few(int nq, int per) const { return nq * per <= few_max; }
+  __device__ __forceinline__ size_t few_row(int seq, int kvh, int nkv, int r) const {
+    return ((size_t)seq * nkv + kvh) * few_tiles * kFewRows + r;
+  }
 };
 
 // -------------------------------------------------------------------- one row --
@@ -342,13 +346,14 @@ __device__ __forceinline__ bool finite4(f4 x) {
 
 // -------------------------------------------------------------------- few rows --
 
-// At most 16 rows a kv head: one token of a sequence, or a verify batch.  Block
-// (split, kv head, sequence); the keys go to the waves 32 at a time (16 of f32), straight from
-// the pages into the operands (each is read once, so there is nothing to stage),
-// and the waves' softmaxes are joined in LDS.  Bound by memory: the next step's
-// page ids, keys and values are on their way while a step is worked on, and f32
-// values go into the f32 instructions as they come (their rate is four times what
-// memory gives; cutting them costs more).
+// At most 64 rows a kv head: one token of a sequence, or a verify batch.  Block
+// (split, tile of 16 rows, kv head; sequence); the keys go to the waves 32 at a time (16
+// of f32), straight from the pages into the operands (a tile reads each once, so there
+// is nothing to stage), and the waves' softmaxes are joined in LDS.  Bound by memory:
+// the next step's page ids, keys and values are on their way while a step is worked on,
+// and f32 values go into the f32 instructions as they come (their rate is four times
+// what memory gives; cutting them costs more).  The tiles of one split run side by side
+// on one XCD (blocks 8 apart), whose L2 gives the later ones the same keys.
 template <class T, int HC>  // HC: head size in steps of 32, rounded up
 __global__ __launch_bounds__(256, HC <= 4 ? 3 : 1) void k_few(AttnArgs a, LayerView<T> kv, BatchView b, Splits sl, bool vec) {
   using F = Form<T>;
@@ -359,22 +364,24 @@ __global__ __launch_bounds__(256, HC <= 4 ? 3 : 1) void k_few(AttnArgs a, LayerV
   __shared__ float ml[2][4][16];
   __shared__ f4 part[2][D][64];
   __shared__ uint32_t bad_rows;
-  const int seq = blockIdx.z, kvh = blockIdx.y, split = blockIdx.x, per = a.heads / kv.nkv, hd = kv.hd;
+  const int seq = blockIdx.y, per = a.heads / kv.nkv, hd = kv.hd;
+  const int t0 = (blockIdx.x >> 3) % sl.few_tiles * kFewRows;  // the tile's first row
+  const int unit = (blockIdx.x >> 3) / sl.few_tiles * 8 + (blockIdx.x & 7), kvh = unit % kv.nkv, split = unit / kv.nkv;
   const SeqSpan sp = seq_span(b, seq);
-  const int rows = sp.nq * per;
-  if (rows == 0 || !few_rows(sp.nq, per)) return;
-  const Tile tile = tile_of(sp, 0, kFewRows, per, a.window);
+  const int rows = min(sp.nq * per - t0, kFewRows);
+  if (rows <= 0 || !sl.is_few(sp.nq, per)) return;
+  const Tile tile = tile_of(sp, t0 / kFewRows, kFewRows, per, a.window);
   const Share each = share_of(tile, sl.few.len);
   const int splits = each.count;
   if (split >= splits) return;
   const int lo = tile.lo + split * each.len, hi = min(tile.hi, lo + each.len);
-  const int seen = first_seen(sp.n - sp.nq, a.window);  // no row sees less
-  const size_t row0 = ((size_t)seq * kv.nkv + kvh) * kFewRows;
+  const int seen = first_seen(sp.n - sp.nq + t0 / per, a.window);  // no row sees less
+  const size_t row0 = sl.few_row(seq, kvh, kv.nkv, t0);
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, col = lane & 15, g = lane >> 4;
   const int *table = b.tables + (size_t)seq * b.stride;
   const int mask = (1 << kv.shift) - 1;
   // The row of this lane's column.
-  const int r = min(col, rows - 1), tok = r / per, head = kvh * per + r % per, pos = sp.n - sp.nq + tok;
+  const int r = t0 + min(col, rows - 1), tok = r / per, head = kvh * per + r % per, pos = sp.n - sp.nq + tok;
   const int first = first_seen(pos, a.window);
   const Score score = score_of(a, head);
   // The rows' queries as operands, the same for every wave, lane after lane.
@@ -594,8 +601,8 @@ __global__ __launch_bounds__(256, HC <= 4 ? 3 : 1) void k_few(AttnArgs a, LayerV
   if (bad_rows == 0) return;
   for (int i = wave; i < rows; i += 4)
     if (bad_rows >> i & 1)
-      redo_row(a, kv, table, sp.q0 + i / per, kvh * per + i % per, sp.n - sp.nq + i / per, lo, hi, sl.few,
-               sl.few.at(row0 + i, split), splits > 1);
+      redo_row(a, kv, table, sp.q0 + (t0 + i) / per, kvh * per + (t0 + i) % per, sp.n - sp.nq + (t0 + i) / per, lo, hi,
+               sl.few, sl.few.at(row0 + i, split), splits > 1);
 }
 
 // ------------------------------------------------------------------- many rows --
@@ -642,7 +649,7 @@ __global__ __launch_bounds__(256, HC <= 4 ? 2 : 1) void k_many(AttnArgs a, Layer
   const int rows = sp.nq * per, tiles = (rows + kManyRows - 1) / kManyRows;
   // Kv heads side by side (an XCD keeps those of its own in L2), the longest rows first.
   const int kvh = blockIdx.x % kv.nkv, t = tiles - 1 - (int)(blockIdx.x / kv.nkv);
-  if (t < 0 || few_rows(sp.nq, per)) return;
+  if (t < 0 || sl.is_few(sp.nq, per)) return;
   const Tile tile = tile_of(sp, t, kManyRows, per, a.window);
   const Share each = share_of(tile, sl.many.len);
   const int splits = each.count;
@@ -915,11 +922,11 @@ __global__ __launch_bounds__(32 * kShares) void k_join(AttnArgs a, BatchView b, 
   const int lane = threadIdx.x & 31, w = threadIdx.x >> 5, share = w & (shares - 1);
   const int unit = blockIdx.x * (kShares / shares) + w / shares, j = unit / a.heads, head = unit % a.heads;
   const int per = a.heads / nkv, kvh = head / per, r = j * per + head % per;
-  const bool few = few_rows(sp.nq, per), mine = j < sp.nq;
+  const bool few = sl.is_few(sp.nq, per), mine = j < sp.nq;
   const int R = few ? kFewRows : kManyRows;
   const Parts &parts = few ? sl.few : sl.many;
   const int splits = mine ? share_of(tile_of(sp, r / R, R, per, a.window), parts.len).count : 0;
-  const size_t row = few ? ((size_t)blockIdx.y * nkv + kvh) * kFewRows + r : (size_t)(sp.q0 + j) * a.heads + head;
+  const size_t row = few ? sl.few_row(blockIdx.y, kvh, nkv, r) : (size_t)(sp.q0 + j) * a.heads + head;
   f4 o[2] = {f4{0, 0, 0, 0}, f4{0, 0, 0, 0}};
   float l = 0.0f;
   if (splits > 1) {
@@ -970,24 +977,51 @@ __global__ __launch_bounds__(32 * kShares) void k_join(AttnArgs a, BatchView b, 
 
 // --------------------------------------------------------------------- launch --
 
-// Splits of the key axis: as many as give the chip about `want` blocks, of whole
-// 128 positions, 256 at least.
-int split_len(size_t units, int keys, size_t want) {
-  const size_t n = std::max<size_t>(1, want / std::max<size_t>(units, 1));
-  const size_t len = (keys + n - 1) / n;
-  return (int)std::max<size_t>(256, (len + 127) / 128 * 128);
-}
+constexpr int kFewMax = 64;   // rows a kv head: four tiles read the keys as often from L2, a block of k_many
+                              // has half of its 128 rows idle (9 tokens x 4 heads at 2200 positions, eight
+                              // sequences: f32 90 us there)
+constexpr size_t kFewBlocks = 2048;
+constexpr size_t kManySlots = 512;  // two blocks a CU
 
+// What a tile can read at most: its rows' windows, from a multiple of 64 on.
 int most_keys(const BatchView &b, int window) {
-  // What a tile can read: its rows' windows, from a multiple of 64 on.
   const long long span = window > 0 ? (long long)window + b.max_q + 63 : b.max_kv;
   return (int)std::max(1LL, std::min<long long>(b.max_kv, span));
 }
 
+int whole128(size_t n) { return (int)((n + 127) / 128 * 128); }
+
+// k_many's splits, for sequences at their bounds: the number that lets the chip end
+// soonest.  Tiles near the start of a prompt read few keys, so that blocks of equal
+// rows are not blocks of equal length: while all fit the chip at once the longest
+// counts, beyond that their sum and half of the longest.  Joining costs some 256
+// positions.  Up to 8 tiles stand for all.
+int many_split(size_t units, size_t tiles, int keys, int max_q) {
+  const int samples = (int)std::min<size_t>(tiles, 8);
+  int best_len = std::max(256, whole128(keys));
+  double best = 0.0;
+  for (int n = 1; n <= 16; ++n) {
+    const int len = std::max(256, whole128(((size_t)keys + n - 1) / n));
+    double blocks = 0.0, sum = 0.0, longest = 0.0;
+    for (int i = 0; i < samples; ++i) {
+      const double span = std::max(1.0, keys - (double)max_q * (samples - 1 - i) / samples);
+      const double parts = std::ceil(span / len);
+      blocks += parts;
+      sum += span;
+      longest = std::max(longest, span / parts);
+    }
+    const double scale = (double)units * tiles / samples;
+    const double cost = (blocks * scale <= kManySlots ? longest : std::max(longest, sum * scale / kManySlots + 0.5 * longest)) +
+                        (len < keys ? 256.0 : 0.0);
+    if (n == 1 || cost < best) best = cost, best_len = len;
+  }
+  return best_len;
+}
+
 struct Plan {
   int few_len, many_len, few, many;  // split lengths and counts
-  size_t few_rows, many_rows;
-  bool use_many;
+  int few_max, few_tiles;
+  size_t few_rows, many_rows, many_tiles;
   size_t few_parts() const { return few > 1 ? few * few_rows : 0; }
   size_t many_parts() const { return many > 1 ? many * many_rows : 0; }
 };
@@ -995,38 +1029,51 @@ struct Plan {
 Plan plan_of(int nkv, int heads, int hd, const BatchView &b, int window, size_t work_bytes) {
   Plan p;
   const int per = heads / nkv, keys = most_keys(b, window);
-  const size_t tiles = ((size_t)b.max_q * per + kManyRows - 1) / kManyRows;
+  const size_t rows = (size_t)b.max_q * per, units = (size_t)b.seqs * nkv;
   size_t left = work_bytes / (4 * (size_t)hd + 8);  // parts that fit
-  auto count = [&](int &len, size_t rows) {
+  auto count = [&](int &len, size_t part_rows) {
     int n = (keys + len - 1) / len;
-    const size_t fit = std::max<size_t>(1, left / rows);
+    const size_t fit = std::max<size_t>(1, left / part_rows);
     if ((size_t)n > fit) {
-      len = (int)((((size_t)keys + fit - 1) / fit + 127) / 128 * 128);
+      len = whole128(((size_t)keys + fit - 1) / fit);
       n = (keys + len - 1) / len;
     }
-    if (n > 1) left -= n * rows;
+    if (n > 1) left -= n * part_rows;
     return n;
   };
-  p.use_many = (size_t)b.max_q * per > kFewRows;
-  p.few_rows = (size_t)b.seqs * nkv * kFewRows;
+  // One sequence with a chunk: no launch for what is not there (should it have few
+  // rows all the same, k_many takes them).
+  p.few_max = b.seqs == 1 && rows > kFewMax ? 0 : kFewMax;
+  p.few_tiles = p.few_max ? (int)((std::min<size_t>(rows, kFewMax) + kFewRows - 1) / kFewRows) : 0;
+  p.few_rows = units * p.few_tiles * kFewRows;
   p.many_rows = (size_t)b.tokens * heads;
-  p.few_len = split_len((size_t)b.seqs * nkv, keys, 2048);
-  p.few = count(p.few_len, p.few_rows);
-  p.many_len = split_len((size_t)b.seqs * nkv * tiles, keys, 512);
-  p.many = p.use_many ? count(p.many_len, p.many_rows) : 1;
+  p.many_tiles = rows > (size_t)p.few_max ? (rows + kManyRows - 1) / kManyRows : 0;
+  p.few = p.many = 1;
+  p.few_len = p.many_len = std::max(256, whole128(keys));
+  if (p.few_tiles) {
+    const size_t want = std::max<size_t>(1, kFewBlocks / (units * p.few_tiles));
+    p.few_len = std::max(256, whole128(((size_t)keys + want - 1) / want));
+    p.few = count(p.few_len, p.few_rows);
+  }
+  if (p.many_tiles) {
+    p.many_len = many_split(units, p.many_tiles, keys, b.max_q);
+    p.many = count(p.many_len, p.many_rows);
+  }
   return p;
 }
 
 template <class T, int HC>
 void launch_of(const AttnArgs &a, const LayerView<T> &kv, const BatchView &b, const Plan &p, const Splits &sl, bool vec,
                hipStream_t s) {
-  if (p.use_many) {
-    const size_t tiles = ((size_t)b.max_q * (a.heads / kv.nkv) + kManyRows - 1) / kManyRows;
+  if (p.many_tiles) {
     constexpr size_t lds = many_lds<T, HC>();
     dynamic_lds<k_many<T, HC>>(lds);
-    k_many<T, HC><<<dim3((unsigned)(tiles * kv.nkv), p.many, b.seqs), 256, lds, s>>>(a, kv, b, sl, vec);
+    k_many<T, HC><<<dim3((unsigned)(p.many_tiles * kv.nkv), p.many, b.seqs), 256, lds, s>>>(a, kv, b, sl, vec);
   }
-  k_few<T, HC><<<dim3(p.few, kv.nkv, b.seqs), 256, 0, s>>>(a, kv, b, sl, vec);
+  if (p.few_tiles) {
+    const unsigned units = ((unsigned)p.few * kv.nkv + 7) / 8 * 8;
+    k_few<T, HC><<<dim3(units * p.few_tiles, b.seqs), 256, 0, s>>>(a, kv, b, sl, vec);
+  }
 }
 
 }  // namespace
@@ -1041,6 +1088,8 @@ void launch_paged_attention(const AttnArgs &a, const LayerView<T> &kv, const Bat
                             size_t work_bytes, hipStream_t s) {
   const Plan p = plan_of(kv.nkv, a.heads, kv.hd, b, a.window, work_bytes);
   Splits sl;
+  sl.few_max = p.few_max;
+  sl.few_tiles = p.few_tiles;
   sl.few = Parts{p.few_len, p.few, static_cast<float *>(work), nullptr};
   sl.many = Parts{p.many_len, p.many, sl.few.o + p.few_parts() * kv.hd, nullptr};
   sl.few.ml = reinterpret_cast<float2 *>(sl.many.o + p.many_parts() * kv.hd);
@@ -1055,7 +1104,7 @@ void launch_paged_attention(const AttnArgs &a, const LayerView<T> &kv, const Bat
   }
   if (p.few > 1 || p.many > 1) {
     // By what most rows have.
-    const int most = p.use_many ? p.many : p.few;
+    const int most = p.many_tiles ? p.many : p.few;
     int shares = 1;
     while (shares < kShares && 4 * shares < most) shares *= 2;
     const int rows = kShares / shares;
