@@ -994,13 +994,14 @@ int whole128(size_t n) { return (int)((n + 127) / 128 * 128); }
 // k_many's splits, for sequences at their bounds: the number that lets the chip end
 // soonest.  Tiles near the start of a prompt read few keys, so that blocks of equal
 // rows are not blocks of equal length: while all fit the chip at once the longest
-// counts, beyond that their sum and half of the longest.  Joining costs some 256
-// positions.  Up to 8 tiles stand for all.
-int many_split(size_t units, size_t tiles, int keys, int max_q) {
+// counts, beyond that their sum and half of the longest.  A split's parts, written
+// and joined, cost about 128 positions (1024 rows x 32 heads: 8 us of 230 for 2560
+// positions).  Up to 8 tiles stand for all; `fit`: parts that the scratch holds.
+int many_split(size_t units, size_t tiles, int keys, int max_q, size_t fit) {
   const int samples = (int)std::min<size_t>(tiles, 8);
   int best_len = std::max(256, whole128(keys));
   double best = 0.0;
-  for (int n = 1; n <= 16; ++n) {
+  for (int n = 1; n <= (int)std::min<size_t>(fit, 16); ++n) {
     const int len = std::max(256, whole128(((size_t)keys + n - 1) / n));
     double blocks = 0.0, sum = 0.0, longest = 0.0;
     for (int i = 0; i < samples; ++i) {
@@ -1012,7 +1013,7 @@ int many_split(size_t units, size_t tiles, int keys, int max_q) {
     }
     const double scale = (double)units * tiles / samples;
     const double cost = (blocks * scale <= kManySlots ? longest : std::max(longest, sum * scale / kManySlots + 0.5 * longest)) +
-                        (len < keys ? 256.0 : 0.0);
+                        (len < keys ? 128.0 * n : 0.0);
     if (n == 1 || cost < best) best = cost, best_len = len;
   }
   return best_len;
@@ -1056,7 +1057,7 @@ Plan plan_of(int nkv, int heads, int hd, const BatchView &b, int window, size_t 
     p.few = count(p.few_len, p.few_rows);
   }
   if (p.many_tiles) {
-    p.many_len = many_split(units, p.many_tiles, keys, b.max_q);
+    p.many_len = many_split(units, p.many_tiles, keys, b.max_q, left / p.many_rows);
     p.many = count(p.many_len, p.many_rows);
   }
   return p;
@@ -1103,12 +1104,13 @@ void launch_paged_attention(const AttnArgs &a, const LayerView<T> &kv, const Bat
     default: launch_of<T, 8>(a, kv, b, p, sl, vec, s); break;
   }
   if (p.few > 1 || p.many > 1) {
-    // By what most rows have.
-    const int most = p.many_tiles ? p.many : p.few;
+    // Rows that can be split, and shares by what most of them have.
+    const int most = p.many > 1 ? p.many : p.few, per = a.heads / kv.nkv;
+    const int rows = p.many > 1 ? b.max_q : std::min(b.max_q, std::max(kFewMax / per, 1));
     int shares = 1;
     while (shares < kShares && 4 * shares < most) shares *= 2;
-    const int rows = kShares / shares;
-    k_join<<<dim3((unsigned)((b.max_q * a.heads + rows - 1) / rows), b.seqs), 32 * kShares, 0, s>>>(a, b, sl, kv.nkv, kv.hd,
+    const int block = kShares / shares;
+    k_join<<<dim3((unsigned)((rows * a.heads + block - 1) / block), b.seqs), 32 * kShares, 0, s>>>(a, b, sl, kv.nkv, kv.hd,
                                                                                                    shares, vec);
   }
 }
