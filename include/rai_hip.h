@@ -306,7 +306,7 @@ typedef enum rai_cache_type { RAI_CACHE_F32 = 0, RAI_CACHE_F16 = 1, RAI_CACHE_BF
  * v [layers][pages][kv_heads][head_dim][page_size] (a head's values lie
  * dimension by dimension, as in the model's own cache) of `type`, 16-byte
  * aligned.  page_size is a power of two from 16 to 1024, head_dim a multiple of
- * 8 up to 256. */
+ * 8 up to 256, kv_heads at most 4096, layers 65535. */
 typedef struct rai_pages {
   void *k, *v;
   size_t layers, pages, page_size, kv_heads, head_dim;
@@ -319,7 +319,8 @@ typedef struct rai_pages {
  * (q_start[s+1] - q_start[s]) + j.  Rows in front of the first sequence and
  * behind the last are nobody's: they are not touched.  max_q bounds the new
  * tokens of a sequence and max_kv its length (they size the launch; lengths
- * past them or past the table are cut). */
+ * past them or past the table are cut).  At most 65535 sequences and 2^24 - 1 rows
+ * a call. */
 typedef struct rai_page_batch {
   const int32_t *tables; /* [seqs][table_stride] page ids */
   size_t table_stride;
@@ -358,7 +359,7 @@ int rai_rope_frequencies(int scaling, double theta, size_t rot_dim, double facto
  * their sequences' pages, rounded once (to nearest, ties to even) to the cache's
  * type.  q, k and v hold a row per token, rows q_stride, k_stride and v_stride
  * floats apart ([heads][head_dim] or [kv_heads][head_dim] each); q_out rows lie
- * q_out_stride apart and may be q itself (same stride).  heads == 0: no queries
+ * q_out_stride apart and may be q itself (same stride), but no other of the inputs.  heads == 0: no queries
  * (q and q_out are not read).  rope == NULL: nothing turns.  Rows whose position
  * is negative or has no page are rotated and not stored.  Two rows of one batch
  * at the same slot: one of them is kept. */
@@ -366,7 +367,8 @@ int rai_paged_store_dev(const rai_pages *pages, size_t layer, const rai_page_bat
                         float *q_out, size_t q_out_stride, const float *q, size_t q_stride, size_t heads,
                         const float *k, size_t k_stride, const float *v, size_t v_stride, void *stream);
 
-/* score = q . k * scale; with softcap > 0: softcap * tanh(score / softcap); with
+/* score = q . k * scale; with softcap (1e-30 to 1e30; 0: off): softcap * tanh(score
+ * / softcap); with
  * slopes (device, [heads]): minus slopes[h] * (row's position - key's position).
  * window > 0: a row sees the last `window` positions up to its own. */
 typedef struct rai_attention_options {
@@ -379,7 +381,8 @@ typedef struct rai_attention_options {
  * (keys and values of the rows themselves are in the pages: rai_paged_store_dev
  * first): out row = sum_j softmax_j(score) v_j over the positions it sees, heads /
  * kv_heads query heads on each kv head.  f32 accuracy for every cache type.  A row
- * that sees nothing becomes zeros.  What a row does not see does not reach it,
+ * that sees nothing becomes zeros.  out must not overlap q; tokens * heads is at most
+ * 2^24 - 1.  What a row does not see does not reach it,
  * NaN and infinities included.
  * work: scratch of the call (16-byte aligned), with which long contexts of few
  * rows are split over the chip; rai_paged_attention_workspace gives the size that

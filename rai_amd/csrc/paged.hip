@@ -346,6 +346,7 @@ bool check_batch(const rai_page_batch *b, const rai_pages *p, BatchView *v) {
   if (b->seqs > 65535) fail(RAI_E_SHAPE, "at most 65535 sequences");
   if (b->tokens > INT32_MAX / 2 || b->table_stride > INT32_MAX || b->max_kv > INT32_MAX / 2)
     fail(RAI_E_SHAPE, "dimensions overflow");
+  if (b->tokens >= size_t(1) << 24) fail(RAI_E_SHAPE, "at most 2^24 - 1 rows in one call");
   const size_t most = std::min<size_t>(b->max_kv, b->table_stride * p->page_size);
   *v = BatchView{b->tables, b->table_stride, b->q_start, b->kv_len, (int)b->seqs, (int)b->tokens,
                  (int)std::min(b->max_q, b->tokens), (int)most};
@@ -393,7 +394,8 @@ void check_rows_heads(const BatchView &b, size_t heads) {
 void check_options(const rai_attention_options *o) {
   if (!o) fail(RAI_E_ARG, "null argument");
   if (!std::isfinite(o->scale)) fail(RAI_E_ARG, "scale must be finite");
-  if (!std::isfinite(o->softcap) || o->softcap < 0.0f) fail(RAI_E_ARG, "softcap must be finite and not negative");
+  if (!(o->softcap == 0.0f || (o->softcap >= 1e-30f && o->softcap <= 1e30f)))
+    fail(RAI_E_ARG, "softcap must be 0 or from 1e-30 to 1e30");
 }
 
 int window_of(const rai_attention_options *o) { return (int)std::min<size_t>(o->window, INT32_MAX / 2); }
@@ -498,6 +500,7 @@ int rai_paged_attention_dev(float *out, size_t out_stride, const float *q, size_
     rai::check_rows_heads(b, heads);
     rai::check_rows(q, q_stride, heads, pages->head_dim, "q");
     rai::check_rows(out, out_stride, heads, pages->head_dim, "out");
+    if (out == q) rai::fail(RAI_E_ARG, "out must not be q");
     if (!work && work_bytes) rai::fail(RAI_E_ARG, "null argument");
     if ((uintptr_t)work % 16) rai::fail(RAI_E_ARG, "work must be 16-byte aligned");
     const rai::AttnArgs a{q, out, q_stride, out_stride, (int)heads, options->scale, options->softcap,

@@ -132,10 +132,11 @@ struct Splits {
 // One row of one head by one wave: positions lo .. hi - 1 of the sequence whose
 // table row is `table`, lane t holding key base + t and dimensions t, t + 64, ...
 // of the output.  Keys that are not there or masked are not read into the sums at
-// all, whatever they hold.  m is in the log2 domain.
+// all, whatever they hold.  m is in the log2 domain; o is the weighted mean so far
+// (a sum of large values could leave f32's range), l the sum of the weights.
 template <class T>
-__device__ __forceinline__ void wave_row(const AttnArgs &a, const LayerView<T> &kv, const int *table, int head, const float *q, int pos,
-                         int lo, int hi, float &m, float &l, float (&o)[4]) {
+__device__ __forceinline__ void wave_row(const AttnArgs &a, const LayerView<T> &kv, const int *table, int head,
+                                         const float *q, int pos, int lo, int hi, float &m, float &l, float (&o)[4]) {
   const int lane = threadIdx.x & 63, hd = kv.hd, kvh = head / (a.heads / kv.nkv), mask = (1 << kv.shift) - 1;
   const Score score = score_of(a, head);
   m = -INFINITY;
@@ -155,13 +156,12 @@ __device__ __forceinline__ void wave_row(const AttnArgs &a, const LayerView<T> &
     float mn = fmaxf(m, wave_max(s));
     if (__any(s != s)) mn = NAN;
     if (mn == -INFINITY) continue;
-    const float scale = exp2f(m - mn), p = exp2f(s - mn);
-    l = l * scale + wave_sum(p);
+    const float p = exp2f(s - mn), old = l * exp2f(m - mn), sum = old + wave_sum(p), inv = 1.0f / sum;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) o[i] *= scale;
+    for (int i = 0; i < 4; ++i) o[i] *= old * inv;
     for (int t = 0; t < 64 && base + t < hi; ++t) {
       const int pg = __shfl(page, t);
-      const float pt = __shfl(p, t);
+      const float pt = __shfl(p, t) * inv;
       if (pg < 0) continue;
       const T *v = kv.v + value_at(pg, kvh, (base + t) & mask, kv.nkv, hd, kv.shift);
 #pragma unroll
@@ -169,6 +169,7 @@ __device__ __forceinline__ void wave_row(const AttnArgs &a, const LayerView<T> &
         if (lane + 64 * i < hd) o[i] = fmaf(pt, to_f32(v[(size_t)(lane + 64 * i) << kv.shift]), o[i]);
     }
     m = mn;
+    l = sum;
   }
 }
 
@@ -184,12 +185,19 @@ __device__ __forceinline__ void redo_row(const AttnArgs &a, const LayerView<T> &
   float *out = a.out + (size_t)row * a.out_stride + (size_t)head * kv.hd;
   if (split) {
     out = parts.o + at * kv.hd;
-    if (lane == 0) parts.ml[at] = make_float2(m, l);
-    l = 1.0f;
+    // The sum as parts hold it; where that leaves f32's range, the mean with all weight in the maximum.
+    bool over = false;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) over = over || (fabsf(o[i]) < INFINITY && !(fabsf(o[i] * l) < INFINITY));
+    over = __any(over);
+    if (lane == 0) parts.ml[at] = over ? make_float2(m + log2f(l), 1.0f) : make_float2(m, l);
+    if (!over)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) o[i] *= l;
   }
 #pragma unroll
   for (int i = 0; i < 4; ++i)
-    if (lane + 64 * i < kv.hd) out[lane + 64 * i] = l == 0.0f ? 0.0f : o[i] / l;
+    if (lane + 64 * i < kv.hd) out[lane + 64 * i] = o[i];
 }
 
 // ------------------------------------------------------------- 16-bit operands --
@@ -916,7 +924,6 @@ __global__ __launch_bounds__(256, HC <= 4 ? 2 : 1) void k_many(AttnArgs a, Layer
 constexpr int kShares = 16;
 __global__ __launch_bounds__(32 * kShares) void k_join(AttnArgs a, BatchView b, Splits sl, int nkv, int hd, int shares,
                                                        bool vec) {
-  __shared__ float ls[kShares];
   __shared__ f4 part[kShares][64];
   const SeqSpan sp = seq_span(b, blockIdx.y);
   const int lane = threadIdx.x & 31, w = threadIdx.x >> 5, share = w & (shares - 1);
@@ -928,50 +935,49 @@ __global__ __launch_bounds__(32 * kShares) void k_join(AttnArgs a, BatchView b, 
   const int splits = mine ? share_of(tile_of(sp, r / R, R, per, a.window), parts.len).count : 0;
   const size_t row = few ? sl.few_row(blockIdx.y, kvh, nkv, r) : (size_t)(sp.q0 + j) * a.heads + head;
   f4 o[2] = {f4{0, 0, 0, 0}, f4{0, 0, 0, 0}};
-  float l = 0.0f;
   if (splits > 1) {
     const float2 *ml = parts.ml + parts.at(row, 0);
     const float *p = parts.o + parts.at(row, 0) * hd + 4 * lane;
-    float top = -INFINITY;
+    float top = -INFINITY, l = 0.0f;
 #pragma unroll 4
     for (int s = lane; s < splits; s += 32) top = fmaxf(top, ml[s].x);
 #pragma unroll
     for (int d = 16; d; d >>= 1) top = fmaxf(top, __shfl_xor(top, d));
+    auto weight = [&](float2 x) { return x.x == top ? 1.0f : __builtin_amdgcn_exp2f(x.x - top); };
+#pragma unroll 4
+    for (int s = lane; s < splits; s += 32) l += weight(ml[s]) * ml[s].y;
+#pragma unroll
+    for (int d = 16; d; d >>= 1) l += __shfl_xor(l, d);
+    const float inv = l == 0.0f ? 0.0f : 1.0f / l;
 #pragma unroll 8
     for (int s = share; s < splits; s += shares) {
-      const float2 x = ml[s];
-      const float weight = x.x == top ? 1.0f : __builtin_amdgcn_exp2f(x.x - top);
-      l += weight * x.y;
+      const float w = weight(ml[s]) * inv;
 #pragma unroll
       for (int i = 0; i < 2; ++i)
-        if (4 * lane + 128 * i < hd) o[i] += *reinterpret_cast<const f4 *>(p + (size_t)s * hd + 128 * i) * weight;
+        if (4 * lane + 128 * i < hd) o[i] += *reinterpret_cast<const f4 *>(p + (size_t)s * hd + 128 * i) * w;
     }
   }
   if (shares > 1) {
-    if (lane == 0) ls[w] = l;
     part[w][lane] = o[0];
     part[w][lane + 32] = o[1];
     __syncthreads();
     if (share) return;
 #pragma unroll 4
     for (int s = 1; s < shares; ++s) {
-      l += ls[w + s];
       o[0] += part[w + s][lane];
       o[1] += part[w + s][lane + 32];
     }
   }
   if (splits < 2) return;
-  const float inv = l == 0.0f ? 0.0f : 1.0f / l;
   float *out = a.out + (size_t)(sp.q0 + j) * a.out_stride + (size_t)head * hd;
 #pragma unroll
   for (int i = 0; i < 2; ++i) {
     const int e = 4 * lane + 128 * i;
     if (e >= hd) continue;
-    const f4 y = o[i] * inv;
     if (vec)
-      *reinterpret_cast<f4 *>(out + e) = y;
+      *reinterpret_cast<f4 *>(out + e) = o[i];
     else
-      for (int k = 0; k < 4; ++k) out[e + k] = y[k];
+      for (int k = 0; k < 4; ++k) out[e + k] = o[i][k];
   }
 }
 

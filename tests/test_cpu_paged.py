@@ -39,14 +39,14 @@ BAD_PAGES = [
     (dict(page_size=0), "RAI_E_SHAPE", "page_size"), (dict(head_dim=0), "RAI_E_SHAPE", "head_dim"),
     (dict(head_dim=12), "RAI_E_SHAPE", "head_dim"), (dict(head_dim=264), "RAI_E_SHAPE", "head_dim"),
     (dict(layers=0), "RAI_E_SHAPE", "empty"), (dict(pages=0), "RAI_E_SHAPE", "empty"),
-    (dict(kv_heads=0), "RAI_E_SHAPE", "empty"), (dict(pages=1 << 31), "RAI_E_SHAPE", "overflow"),
+    (dict(kv_heads=0), "RAI_E_SHAPE", "empty"), (dict(kv_heads=4097), "RAI_E_SHAPE", "overflow"), (dict(pages=1 << 31), "RAI_E_SHAPE", "overflow"),
     (dict(k=AT + 8), "RAI_E_ARG", "aligned"), (dict(v=AT + 2), "RAI_E_ARG", "aligned"),
 ]
 BAD_BATCH = [
     (dict(tables=None), "RAI_E_ARG", "null"), (dict(q_start=None), "RAI_E_ARG", "null"),
     (dict(kv_len=None), "RAI_E_ARG", "null"), (dict(table_stride=0), "RAI_E_SHAPE", "table_stride"),
     (dict(seqs=65536), "RAI_E_SHAPE", "65535"), (dict(tokens=1 << 31), "RAI_E_SHAPE", "overflow"),
-    (dict(max_kv=1 << 31), "RAI_E_SHAPE", "overflow"), (dict(table_stride=1 << 31), "RAI_E_SHAPE", "overflow"),
+    (dict(tokens=1 << 24), "RAI_E_SHAPE", "2^24"), (dict(max_kv=1 << 31), "RAI_E_SHAPE", "overflow"), (dict(table_stride=1 << 31), "RAI_E_SHAPE", "overflow"),
 ]
 
 
@@ -57,7 +57,7 @@ def _store(rai, pages=None, layer=0, batch=None, rope="ok", q_out=AT, qo_ld=256,
                                          heads, k, k_ld, v, v_ld, None)
 
 
-def _attend(rai, pages=None, layer=0, batch=None, opts=None, out=AT, o_ld=256, q=AT, q_ld=256, heads=4, work=None, n=0):
+def _attend(rai, pages=None, layer=0, batch=None, opts=None, out=2 * AT, o_ld=256, q=AT, q_ld=256, heads=4, work=None, n=0):
     opts = opts or rai.AttentionOptions(0.125, 0.0, 0, None)
     return rai.lib().rai_paged_attention_dev(out, o_ld, q, q_ld, heads, pages or _pages(rai), layer,
                                              batch or _batch(rai), opts, work, n, None)
@@ -90,18 +90,20 @@ def test_refused_stores(rai):
     for name, n in (("q_ld", 255), ("qo_ld", 255), ("k_ld", 127), ("v_ld", 127)):
         _refused(rai, _store(rai, **{name: n}), "RAI_E_SHAPE", "overlap")
     _refused(rai, _store(rai, q_ld=300), "RAI_E_SHAPE", "in place")
-    _refused(rai, _store(rai, pages=None, batch=None, heads=65536), "RAI_E_SHAPE", "overflow")
+    _refused(rai, _store(rai, pages=None, batch=None, heads=16385), "RAI_E_SHAPE", "overflow")
 
 
 def test_refused_attention(rai):
     O = rai.AttentionOptions
     _refused(rai, _attend(rai, layer=2), "RAI_E_RANGE", "layer")
-    for heads in (0, 3, 65536):
+    for heads in (0, 3, 16386):
         _refused(rai, _attend(rai, heads=heads, q_ld=1 << 24, o_ld=1 << 24), "RAI_E_SHAPE", "heads")
     for scale in (math.nan, math.inf):
         _refused(rai, _attend(rai, opts=O(scale, 0.0, 0, None)), "RAI_E_ARG", "scale")
-    for cap in (-1.0, math.nan, math.inf):
+    for cap in (-1.0, math.nan, math.inf, 1e-31, 1e31):
         _refused(rai, _attend(rai, opts=O(1.0, cap, 0, None)), "RAI_E_ARG", "softcap")
+    _refused(rai, _attend(rai, out=AT), "RAI_E_ARG", "out must not be q")
+    _refused(rai, _attend(rai, batch=_batch(rai, tokens=1 << 22)), "RAI_E_SHAPE", "rows x heads")
     _refused(rai, _attend(rai, out=None), "RAI_E_ARG", "null")
     _refused(rai, _attend(rai, q=None), "RAI_E_ARG", "null")
     _refused(rai, _attend(rai, q_ld=255), "RAI_E_SHAPE", "overlap")

@@ -290,6 +290,118 @@ def test_attention_calls_on_two_streams_and_in_a_graph(rai):
         rai._check(L.rai_stream_destroy(s))
 
 
+@pytest.mark.parametrize("cache", CACHES)
+@pytest.mark.parametrize("news,lengths", [([1], [1]), ([1, 2], [0, 0]), ([3, 200], [0, 0])])
+def test_attention_nothing_cached(rai, cache, news, lengths):
+    """Lengths of zero and one; a table of one page."""
+    pool = Pool(cache, 16, 1, 64, lengths, seed=1)
+    pool.fill(0, lengths)
+    _check_attention(rai, pool, news, lengths, 2, 0.125)
+
+
+@pytest.mark.parametrize("cache", CACHES)
+@pytest.mark.parametrize("nq", [1, 5, 9, 40])
+def test_attention_many_heads_on_one(rai, cache, nq):
+    """70 query heads on a kv head: one token is more rows than the kernel of few rows takes."""
+    pool = Pool(cache, 32, 1, 64, [300, 90], seed=2)
+    pool.fill(0, [300, 90])
+    _check_attention(rai, pool, [nq, 1], [300, 90], 70, 0.125)
+
+
+@pytest.mark.parametrize("cache", ["f32", "bf16"])
+@pytest.mark.parametrize("nq,n", [(1, 900), (70, 900)])
+def test_attention_values_near_the_type_s_largest(rai, cache, nq, n):
+    """Means of values near 3e38 stay finite, split or not."""
+    pool = Pool(cache, 16, 1, 64, [n], seed=3)
+    pool.fill(0, [n])
+    top = encode(np.float32([3e38]), cache)[0]
+    pool.v[:, pool.tables[0]] = top
+    pool.v[:, pool.tables[0], :, ::2] = encode(np.float32([-3e38]), cache)[0]
+    want = decode(np.array([top]), cache)[0]
+    dev, q = Dev(rai), np.random.default_rng(1).standard_normal((nq, 4, 64)).astype(np.float32)
+    pg, batch = dev.pages(pool), dev.batch(pool, [0, nq], [n], nq, nq, n)
+    for work in (None, 0):
+        got = _run_attention(rai, dev, pg, batch, q, 4, 64, rai.AttentionOptions(0.125, 0.0, 0, None), work=work)
+        # The weights' sum is off by a half step a key at most, and so is their weighted sum.
+        assert (np.abs(got[:, :, 1::2].astype(np.float64) / want - 1) <= 2 * (n + 16) * EPS32).all()
+        assert (np.abs(got[:, :, ::2].astype(np.float64) / -want - 1) <= 2 * (n + 16) * EPS32).all()
+
+
+@pytest.mark.parametrize("cache", CACHES)
+def test_chunk_attention_in_a_graph(rai, cache):
+    """A chunk's kernels, their scratch and more than 64 KB of LDS captured; replays on other queries with
+    eager calls between them."""
+    L, P, heads, hd, nq, n = rai.lib(), ctypes.c_void_p, 4, 128, 70, 1300
+    pool = Pool(cache, 64, 2, hd, [n], seed=9)
+    pool.fill(0, [n])
+    dev, rng = Dev(rai), np.random.default_rng(0)
+    pg, batch = dev.pages(pool), dev.batch(pool, [0, nq], [n], nq, nq, n)
+    opts = rai.AttentionOptions(0.1, 0.0, 0, None)
+    qs = [rng.standard_normal((nq, heads, hd)).astype(np.float32) for _ in range(3)]
+    size = rai.attention_workspace(heads, pg, batch, opts)
+    dq, do, dw = dev.up(qs[0]), dev.up(np.zeros_like(qs[0])), rai.DeviceArray(max(size, 16))
+    stream, graph, ex = P(), P(), P()
+    rai._check(L.rai_stream_create(ctypes.byref(stream)))
+    gc.collect()
+    gc.disable()
+    try:
+        assert L.hipStreamBeginCapture(stream, 1) == 0
+        rc = L.rai_paged_attention_dev(do.ptr, heads * hd, dq.ptr, heads * hd, heads, pg, 0, batch, opts, dw.ptr, size,
+                                       stream)
+        assert L.hipStreamEndCapture(stream, ctypes.byref(graph)) == 0
+    finally:
+        gc.enable()
+    rai._check(rc)
+    assert L.hipGraphInstantiate(ctypes.byref(ex), graph, None, None, ctypes.c_size_t(0)) == 0
+    for i in (0, 1, 2, 0):
+        want, tol = attend(pool, 0, (0, nq, n), 0, qs[i], heads, 0.1)
+        rai._check(L.rai_memcpy_h2d(dq.ptr, qs[i].ctypes.data, qs[i].nbytes))
+        assert L.hipGraphLaunch(ex, stream) == 0
+        rai._check(L.rai_stream_synchronize(stream))
+        got = do.to_host(np.float32, qs[i].size).reshape(qs[i].shape)
+        assert (np.abs(got - want) <= tol).all()
+        eager = _run_attention(rai, dev, pg, batch, qs[i], heads, hd, opts)
+        assert np.array_equal(eager.view(np.uint32), got.view(np.uint32))
+    assert L.hipGraphExecDestroy(ex) == 0 and L.hipGraphDestroy(graph) == 0
+    rai._check(L.rai_stream_destroy(stream))
+
+
+def test_offsets_past_32_bits(rai):
+    """Pages whose elements lie past 2^32 of the pool: stored, attended, forked and moved there."""
+    heads, kv_heads, hd, page, n, high = 4, 2, 64, 64, 150, (1 << 32) // (2 * 64 * 64) + 3
+    small = Pool("bf16", page, kv_heads, hd, [n], seed=4)
+    rng = np.random.default_rng(6)
+    k, v = rng.standard_normal((2, n, kv_heads * hd)).astype(np.float32)
+    q = rng.standard_normal((n, heads, hd)).astype(np.float32)
+    for p in range(n):
+        small.put(0, 0, p, k[p].reshape(kv_heads, hd), v[p].reshape(kv_heads, hd))
+    count = high + 8
+    dk, dv = (rai.DeviceArray(2 * count * kv_heads * page * hd) for _ in range(2))
+    pg = rai.Pages(dk.ptr, dv.ptr, 1, count, page, kv_heads, hd, rai.CACHE_BF16)
+    dev, L = Dev(rai), rai.lib()
+    tables = dev.up(np.int32([[high, high + 2, high + 1]]))
+    batch = rai.PageBatch(tables.ptr, 3, dev.up(np.int32([0, n])).ptr, dev.up(np.int32([n])).ptr, 1, n, n, n)
+    rai._check(L.rai_paged_store_dev(pg, 0, batch, None, None, 0, None, 0, 0, dev.up(k).ptr, kv_heads * hd, dev.up(v).ptr,
+                                     kv_heads * hd, None))
+    opts = rai.AttentionOptions(0.125, 0.0, 0, None)
+    want, tol = attend(small, 0, (0, n, n), 0, q, heads, 0.125)
+    got = _run_attention(rai, dev, pg, batch, q, heads, hd, opts)
+    assert (np.abs(got - want) <= tol).all()
+    # Two children of a sequence of 150 positions, the second's last page to high + 5, then that to high + 7.
+    out = [dev.up(np.zeros(m, np.int32)) for m in (6, 2, 2)]
+    rai._check(L.rai_paged_fork_dev(pg, tables.ptr, 3, dev.up(np.int32([n])).ptr, 1, dev.up(np.int32([0, 0])).ptr,
+                                    dev.up(np.int32([high + 4, high + 5])).ptr, 2, *[o.ptr for o in out], None))
+    rai._check(L.rai_paged_move_dev(pg, dev.up(np.int32([high + 5])).ptr, dev.up(np.int32([high + 7])).ptr, 1, out[0].ptr,
+                                    6, None))
+    rai._check(L.rai_device_synchronize())
+    assert out[0].to_host(np.int32, 6).tolist() == [high, high + 2, high + 1, high, high + 2, high + 7]
+    for nq in (1, n):
+        two = rai.PageBatch(out[0].ptr, 3, dev.up(np.int32([0, nq, 2 * nq])).ptr, out[1].ptr, 2, 2 * nq, nq, n)
+        got = _run_attention(rai, dev, pg, two, np.concatenate([q[n - nq:]] * 2), heads, hd, opts)
+        for half in (got[:nq], got[nq:]):
+            assert (np.abs(half - want[n - nq:]) <= tol[n - nq:]).all()
+
+
 # ------------------------------------------------------------------- store --
 
 def _check_store(rai, cache, page, heads, kv_heads, hd, news, lengths, rot, interleaved, gain=1.0, front=0, back=0,
