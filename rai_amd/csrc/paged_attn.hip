@@ -107,7 +107,6 @@ __device__ __forceinline__ Share share_of(const Tile &t, int len) {
 constexpr int kFewRows = 16;    // a tile of k_few
 constexpr int kManyRows = 128;  // a tile of k_many
 
-
 // Sequences of at most few_max rows a kv head go to k_few, others to k_many.  How
 // the key axis is split, and where the parts of a row's softmax lie: [row][split] x hd
 // values, and maximum and sum.  k_few's rows are 16 few_tiles to a (sequence, kv head),
@@ -359,9 +358,12 @@ __device__ __forceinline__ bool finite4(f4 x) {
 // of f32), straight from the pages into the operands (a tile reads each once, so there
 // is nothing to stage), and the waves' softmaxes are joined in LDS.  Bound by memory:
 // the next step's page ids, keys and values are on their way while a step is worked on,
-// and f32 values go into the f32 instructions as they come (their rate is four times
-// what memory gives; cutting them costs more).  The tiles of one split run side by side
-// on one XCD (blocks 8 apart), whose L2 gives the later ones the same keys.
+// and f32 values go into the f32 instructions as they come (64 a step of 16 keys, four
+// times as fast as memory delivers; cutting the values took some 700 vector instructions
+// a step).  The tiles of one split run side by side on one XCD (blocks 8 apart), whose L2
+// gives the later ones the same keys.  32 sequences of up to 4096 positions, 32 heads on
+// 8 of 128 dimensions, bf16: 79 us, 4.5 TB/s; 9 tokens of 8 sequences, 16 heads, f32:
+// 77 us, 4.1 TB/s; one token at 200 positions: 10 us, all of it latency.
 template <class T, int HC>  // HC: head size in steps of 32, rounded up
 __global__ __launch_bounds__(256, HC <= 4 ? 3 : 1) void k_few(AttnArgs a, LayerView<T> kv, BatchView b, Splits sl, bool vec) {
   using F = Form<T>;
@@ -919,8 +921,9 @@ __global__ __launch_bounds__(256, HC <= 4 ? 2 : 1) void k_many(AttnArgs a, Layer
 
 // Splits of a row joined: 32 lanes x 4 dimensions (twice over for heads past 128)
 // by `shares` (1 to 16, a power of two) that take the splits in turn; a block has 16
-// / shares rows.  Block (rows, sequence).  Bound by the latency of its loads: all of
-// a share's maxima are read at once, and its parts eight at a time.
+// / shares rows.  Block (rows, sequence).  Bound by the latency of its loads: a row's
+// maxima are read first, a share's parts eight at a time.  32 rows of 129 parts: 10 us;
+// 32768 of two: 16.
 constexpr int kShares = 16;
 __global__ __launch_bounds__(32 * kShares) void k_join(AttnArgs a, BatchView b, Splits sl, int nkv, int hd, int shares,
                                                        bool vec) {
