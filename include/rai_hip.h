@@ -295,7 +295,8 @@ int rai_attention_head_dev(float *out, const float *q, const float *k, const flo
  * All pointers in the structures are device pointers, and so are the calls'
  * arrays; the structures themselves are host memory, read during the call.
  * The calls are asynchronous on `stream`, allocate nothing, keep nothing
- * between calls and may be captured into a graph.  Entries of device arrays
+ * between calls and may be captured into a graph; stream and pointers belong to
+ * the current device.  Entries of device arrays
  * cannot fail a call; they are bounded instead: a page id outside 0..pages-1
  * is a page that is not there (nothing is read from it or written to it, and
  * its keys are not seen), row starts and lengths are cut to the bounds given
@@ -318,8 +319,9 @@ typedef struct rai_pages {
  * of its kv_len[s] ones: row q_start[s] + j is position kv_len[s] -
  * (q_start[s+1] - q_start[s]) + j.  Rows in front of the first sequence and
  * behind the last are nobody's: they are not touched.  max_q bounds the new
- * tokens of a sequence and max_kv its length (they size the launch; lengths
- * past them or past the table are cut).  At most 65535 sequences and 2^24 - 1 rows
+ * tokens of a sequence and max_kv its length; they size the launch: rows past max_q
+ * are left out, as if the sequence's rows ended there, and a length past max_kv or
+ * past the table becomes that.  At most 65535 sequences and 2^24 - 1 rows
  * a call. */
 typedef struct rai_page_batch {
   const int32_t *tables; /* [seqs][table_stride] page ids */

@@ -755,6 +755,94 @@ def test_beam_in_a_graph(rai):
 
 # ---------------------------------------------------------------- together --
 
+def test_a_step_in_a_graph(rai):
+    """Selection, fork, store, attention and a move captured as one graph and replayed on other logits and
+    rows, with eager runs of the same step on other buffers between the replays: equal bits."""
+    L, P = rai.lib(), ctypes.c_void_p
+    heads, kv_heads, hd, page, beams, vocab, n, stride = 8, 2, 64, 16, 4, 5000, 40, 4
+    # No length ends a page: two children of such a sequence would share its last slot, which this step writes.
+    lengths = [n, n - 3, n - 7, 5]
+    rng = np.random.default_rng(3)
+    inputs = [[a.astype(np.float32) for a in (2.0 * rng.standard_normal((beams, vocab)), rng.standard_normal((beams, heads * hd)),
+                                              rng.standard_normal((2, beams, kv_heads * hd)))] for _ in range(3)]
+    scores = np.float32([-1.0, -1.5, -0.5, -2.0])
+    inv, gain = rai.rope_frequencies(rai.ROPE_NONE, 1e4, hd)
+    options = rai.AttentionOptions(0.125, 0.0, 0, None)
+
+    class Step:
+        """Buffers of one step, and the calls."""
+
+        def __init__(self):
+            self.pool = Pool("f16", page, kv_heads, hd, lengths, seed=2, spare=20, stride=stride)
+            self.pool.fill(0, lengths)
+            self.dev = d = Dev(rai)
+            self.pages = d.pages(self.pool)
+            self.logits, self.q, self.kv = (d.up(a) for a in inputs[0])
+            self.scores, self.inv = d.up(scores), d.up(inv)
+            self.tables, self.lengths = d.up(self.pool.tables), d.up(np.int32(lengths))
+            self.parent, self.token, self.score, self.next_len, self.used = (d.up(np.zeros(beams, np.int32)) for _ in range(5))
+            self.fresh = d.up(np.int32(self.pool.spare[:beams]))
+            self.next_tables, self.starts = d.up(np.zeros((beams, stride), np.int32)), d.up(np.int32(np.arange(beams + 1)))
+            self.src, self.dst = d.up(np.int32(self.pool.spare[:1])), d.up(np.int32(self.pool.spare[beams:beams + 1]))
+            self.out = d.up(np.zeros((beams, heads * hd), np.float32))
+            self.batch = rai.PageBatch(self.next_tables.ptr, stride, self.starts.ptr, self.next_len.ptr, beams, beams, 1, n)
+            self.need = rai.beam_workspace(vocab, 1, beams, beams)
+            self.work = rai.DeviceArray(self.need)
+
+        def give(self, values):
+            for to, a in zip((self.logits, self.q, self.kv), values):
+                rai._check(L.rai_memcpy_h2d(to.ptr, a.ctypes.data, a.nbytes))
+            for to, a in zip((self.dev.k, self.dev.v), (self.pool.k, self.pool.v)):
+                rai._check(L.rai_memcpy_h2d(to.ptr, a.ctypes.data, a.nbytes))
+
+        def run(self, stream):
+            rope, w, kw = rai.Rope(self.inv.ptr, hd, 0, gain), heads * hd, kv_heads * hd
+            return [L.rai_beam_select_dev(self.logits.ptr, vocab, vocab, self.scores.ptr, None, 0, 1, beams, beams,
+                                          self.parent.ptr, self.token.ptr, self.score.ptr, self.work.ptr, self.need, stream),
+                    L.rai_paged_fork_dev(self.pages, self.tables.ptr, stride, self.lengths.ptr, beams, self.parent.ptr,
+                                         self.fresh.ptr, beams, self.next_tables.ptr, self.next_len.ptr, self.used.ptr, stream),
+                    L.rai_paged_store_dev(self.pages, 0, self.batch, rope, self.q.ptr, w, self.q.ptr, w, heads, self.kv.ptr,
+                                          kw, self.kv.ptr + 4 * beams * kw, kw, stream),
+                    L.rai_paged_move_dev(self.pages, self.src.ptr, self.dst.ptr, 1, self.next_tables.ptr, beams * stride, stream),
+                    L.rai_paged_attention_dev(self.out.ptr, w, self.q.ptr, w, heads, self.pages, 0, self.batch, options, None,
+                                              0, stream)]
+
+        def results(self):
+            rai._check(L.rai_device_synchronize())
+            ints = [a.to_host(np.int32, beams) for a in (self.parent, self.token, self.next_len, self.used)]
+            return ints + [self.next_tables.to_host(np.int32, beams * stride), self.out.to_host(np.uint32, beams * heads * hd),
+                           *(a.view(np.uint16) for a in self.dev.pool_back(self.pool))]
+
+    captured, eager = Step(), Step()
+    stream, graph, ex = P(), P(), P()
+    rai._check(L.rai_stream_create(ctypes.byref(stream)))
+    gc.collect()
+    gc.disable()
+    try:
+        assert L.hipStreamBeginCapture(stream, 1) == 0
+        rcs = captured.run(stream)
+        assert L.hipStreamEndCapture(stream, ctypes.byref(graph)) == 0
+    finally:
+        gc.enable()
+    assert rcs == [0] * 5, L.rai_last_error()
+    assert L.hipGraphInstantiate(ctypes.byref(ex), graph, None, None, ctypes.c_size_t(0)) == 0
+    seen = []
+    for i in (0, 1, 2, 0, 1):
+        captured.give(inputs[i])
+        eager.give(inputs[i])
+        assert L.hipGraphLaunch(ex, stream) == 0
+        rai._check(L.rai_stream_synchronize(stream))
+        got = captured.results()
+        assert eager.run(None) == [0] * 5
+        for a, b in zip(got, eager.results()):
+            assert np.array_equal(a, b)
+        assert np.isfinite(got[5].view(np.float32)).all()
+        seen.append(tuple(got[0]) + tuple(got[1]))
+    assert len(set(seen)) == 3 and seen[0] == seen[3]
+    assert L.hipGraphExecDestroy(ex) == 0 and L.hipGraphDestroy(graph) == 0
+    rai._check(L.rai_stream_destroy(stream))
+
+
 @pytest.mark.parametrize("cache", CACHES)
 def test_beam_search_over_the_pages(rai, cache):
     """A beam search as a program runs it: the prompt stored and attended as a chunk, then steps of
