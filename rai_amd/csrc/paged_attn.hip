@@ -1003,15 +1003,16 @@ int whole128(size_t n) { return (int)((n + 127) / 128 * 128); }
 // k_many's splits, for sequences at their bounds: the number that lets the chip end
 // soonest.  Tiles near the start of a prompt read few keys, so that blocks of equal
 // rows are not blocks of equal length: while all fit the chip at once the longest
-// counts, beyond that their sum and half of the longest.  A split's parts, written
-// and joined, cost about 128 positions (1024 rows x 32 heads: 8 us of 230 for 2560
-// positions).  Up to 8 tiles stand for all; `fit`: parts that the scratch holds.
-int many_split(size_t units, size_t tiles, int keys, int max_q, size_t fit) {
+// counts, beyond that their sum and half of the longest.  In positions of a block
+// (0.07 to 0.09 us each): the join costs about 100, its launch, and 90 a split for
+// 32768 rows x heads of 128, the parts written and read (1024 rows x 32 heads: 8 us
+// a split).  Up to 8 tiles stand for all; `fit`: parts that the scratch holds.
+int many_split(size_t units, size_t tiles, int keys, int max_q, size_t row_bytes, size_t fit) {
   const int samples = (int)std::min<size_t>(tiles, 8);
-  int best_len = std::max(256, whole128(keys));
+  int best_len = std::max(128, whole128(keys));
   double best = 0.0;
   for (int n = 1; n <= (int)std::min<size_t>(fit, 16); ++n) {
-    const int len = std::max(256, whole128(((size_t)keys + n - 1) / n));
+    const int len = whole128(((size_t)keys + n - 1) / n);
     double blocks = 0.0, sum = 0.0, longest = 0.0;
     for (int i = 0; i < samples; ++i) {
       const double span = std::max(1.0, keys - (double)max_q * (samples - 1 - i) / samples);
@@ -1021,8 +1022,9 @@ int many_split(size_t units, size_t tiles, int keys, int max_q, size_t fit) {
       longest = std::max(longest, span / parts);
     }
     const double scale = (double)units * tiles / samples;
-    const double cost = (blocks * scale <= kManySlots ? longest : std::max(longest, sum * scale / kManySlots + 0.5 * longest)) +
-                        (len < keys ? 128.0 * n : 0.0);
+    const double join = len < keys ? 100.0 + 90.0 * n * (double)row_bytes / (32768.0 * 128 * 4) : 0.0;
+    const double cost =
+        join + (blocks * scale <= kManySlots ? longest : std::max(longest, sum * scale / kManySlots + 0.5 * longest));
     if (n == 1 || cost < best) best = cost, best_len = len;
   }
   return best_len;
@@ -1066,7 +1068,7 @@ Plan plan_of(int nkv, int heads, int hd, const BatchView &b, int window, size_t 
     p.few = count(p.few_len, p.few_rows);
   }
   if (p.many_tiles) {
-    p.many_len = many_split(units, p.many_tiles, keys, b.max_q, left / p.many_rows);
+    p.many_len = many_split(units, p.many_tiles, keys, b.max_q, p.many_rows * hd * 4, left / p.many_rows);
     p.many = count(p.many_len, p.many_rows);
   }
   return p;
