@@ -383,7 +383,7 @@ typedef struct rai_attention_options {
  * (keys and values of the rows themselves are in the pages: rai_paged_store_dev
  * first): out row = sum_j softmax_j(score) v_j over the positions it sees, heads /
  * kv_heads query heads on each kv head.  f32 accuracy for every cache type.  A row
- * that sees nothing becomes zeros.  out must not overlap q; tokens * heads is at most
+ * that sees nothing, or only scores of -inf, becomes zeros.  out must not overlap q; tokens * heads is at most
  * 2^24 - 1.  What a row does not see does not reach it,
  * NaN and infinities included.
  * work: scratch of the call (16-byte aligned), with which long contexts of few
