@@ -989,7 +989,10 @@ __global__ __launch_bounds__(32 * kShares) void k_join(AttnArgs a, BatchView b, 
 constexpr int kFewMax = 64;   // rows a kv head: four tiles read the keys as often from L2, a block of k_many
                               // has half of its 128 rows idle (9 tokens x 4 heads at 2200 positions, eight
                               // sequences: f32 90 us there)
-constexpr size_t kFewBlocks = 2048;
+// Blocks of k_few: pieces that even out sequences of different lengths, or, of one
+// sequence, about as many as the chip holds at once (one token at 32768 positions: 40
+// us with 65 parts a row, 44 with 129, 46 with 43).
+constexpr size_t kFewBlocks = 2048, kFewBlocksOne = 640;
 constexpr size_t kManySlots = 512;  // two blocks a CU
 
 // What a tile can read at most: its rows' windows, from a multiple of 64 on.
@@ -1063,7 +1066,7 @@ Plan plan_of(int nkv, int heads, int hd, const BatchView &b, int window, size_t 
   p.few = p.many = 1;
   p.few_len = p.many_len = std::max(256, whole128(keys));
   if (p.few_tiles) {
-    const size_t want = std::max<size_t>(1, kFewBlocks / (units * p.few_tiles));
+    const size_t want = std::max<size_t>(1, (b.seqs == 1 ? kFewBlocksOne : kFewBlocks) / (units * p.few_tiles));
     p.few_len = std::max(256, whole128(((size_t)keys + want - 1) / want));
     p.few = count(p.few_len, p.few_rows);
   }
