@@ -922,7 +922,7 @@ __global__ __launch_bounds__(256, HC <= 4 ? 2 : 1) void k_many(AttnArgs a, Layer
 // Splits of a row joined: 32 lanes x 4 dimensions (twice over for heads past 128)
 // by `shares` (1 to 16, a power of two) that take the splits in turn; a block has 16
 // / shares rows.  Block (rows, sequence).  Bound by the latency of its loads: a row's
-// maxima are read first, a share's parts eight at a time.  32 rows of 129 parts: 10 us;
+// maxima are read first, a share's parts eight at a time.  32 rows of 65 parts: 8 us;
 // 32768 of two: 16.
 constexpr int kShares = 16;
 __global__ __launch_bounds__(32 * kShares) void k_join(AttnArgs a, BatchView b, Splits sl, int nkv, int hd, int shares,
