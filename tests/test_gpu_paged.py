@@ -225,6 +225,25 @@ def test_attention_bad_entries(rai, cache):
     _check_attention(rai, pool, [3, 2, 40], lengths, 4, 0.125, q_start=[-5, 3, 2, 10 ** 9], max_q=20)
 
 
+@pytest.mark.parametrize("seed", range(24))
+def test_attention_random_batches(rai, seed):
+    """Head layouts, sizes, lengths, options, strides, layers and broken tables, drawn."""
+    r = np.random.default_rng(seed)
+    hd, kv_heads, per = 8 * r.integers(1, 33), int(r.choice([1, 2, 3, 5])), int(r.choice([1, 2, 3, 4, 7, 8, 33]))
+    heads, seqs = kv_heads * per, r.integers(1, 6)
+    news = [int(r.choice([0, 1, 1, 2, 9, 40])) for _ in range(seqs)] + [1]
+    lengths = [max(0, m + int(r.choice([-3, 0, 1, 15, 63, 200, 500]))) for m in news]
+    pool = Pool(CACHES[seed % 3], 16 << r.integers(5), kv_heads, int(hd), lengths, seed=seed, layers=2)
+    pool.fill(1, lengths, std=float(r.choice([0.3, 1.0, 3.0])))
+    for _ in range(seed % 4):
+        pool.tables[r.integers(seqs), r.integers(pool.tables.shape[1])] = int(r.choice([-1, pool.pages, 1 << 30]))
+    slopes = 2.0 ** (-8.0 * np.arange(1, heads + 1) / heads) if r.random() < 0.3 else None
+    _check_attention(rai, pool, news, lengths, heads, float(r.choice([hd ** -0.5, -0.2, 0.5, 0.0])),
+                     softcap=float(r.choice([0.0, 3.0, 25.0])), window=int(r.choice([0, 1, 7, 64, 301])), slopes=slopes,
+                     front=int(r.integers(3)), back=int(r.integers(3)), layer=1, ld=int(heads * hd + r.choice([0, 1, 4])),
+                     out_ld=int(heads * hd + r.choice([0, 3, 4])), works=(None, 0, int(4096 * r.integers(1, 40))))
+
+
 def test_attention_calls_on_two_streams_and_in_a_graph(rai):
     """Two calls in flight with scratch of their own; a captured call replayed on new lengths and queries."""
     L, P, heads, hd = rai.lib(), ctypes.c_void_p, 8, 64
