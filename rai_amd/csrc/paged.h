@@ -71,8 +71,9 @@ struct AttnArgs {
   const float *slopes;
 };
 
-// Bytes of work that launch_paged_attention can use for these bounds.
-size_t paged_attention_work(int nkv, int heads, int hd, const BatchView &b, int window);
+// Bytes of work that launch_paged_attention can use for these bounds and elements of
+// `size` bytes.
+size_t paged_attention_work(int nkv, int heads, int hd, int size, const BatchView &b, int window);
 template <class T>
 void launch_paged_attention(const AttnArgs &a, const LayerView<T> &kv, const BatchView &b, void *work,
                             size_t work_bytes, hipStream_t s);

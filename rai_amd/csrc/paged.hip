@@ -485,8 +485,8 @@ int rai_paged_attention_workspace(size_t heads, const rai_pages *pages, const ra
     *bytes = 0;
     if (!rai::check_batch(batch, pages, &b)) return RAI_OK;
     rai::check_rows_heads(b, heads);
-    *bytes = rai::paged_attention_work((int)pages->kv_heads, (int)heads, (int)pages->head_dim, b,
-                                       rai::window_of(options));
+    *bytes = rai::paged_attention_work((int)pages->kv_heads, (int)heads, (int)pages->head_dim,
+                                       (int)rai::type_bytes(pages->type), b, rai::window_of(options));
   });
 }
 

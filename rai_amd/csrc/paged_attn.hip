@@ -363,16 +363,18 @@ __device__ __forceinline__ bool finite4(f4 x) {
 // a step).  The tiles of one split run side by side on one XCD (blocks 8 apart), whose L2
 // gives the later ones the same keys.  32 sequences of up to 4096 positions, 32 heads on
 // 8 of 128 dimensions, bf16: 79 us, 4.5 TB/s; 9 tokens of 8 sequences, 16 heads, f32:
-// 77 us, 4.1 TB/s; one token at 200 positions: 10 us, all of it latency.
-template <class T, int HC>  // HC: head size in steps of 32, rounded up
-__global__ __launch_bounds__(256, HC <= 4 ? 3 : 1) void k_few(AttnArgs a, LayerView<T> kv, BatchView b, Splits sl, bool vec) {
+// 77 us, 4.1 TB/s.  Short contexts of few heads are all latency, some 6 us and 1.5 to 2
+// a round of the waves: eight waves and no split there (launch_of).
+// HC: head size in steps of 32, rounded up; W: waves.
+template <class T, int HC, int W>
+__global__ __launch_bounds__(64 * W, W > 4 ? 2 : HC <= 4 ? 3 : 1) void k_few(AttnArgs a, LayerView<T> kv, BatchView b, Splits sl, bool vec) {
   using F = Form<T>;
   constexpr int KP = F::KP, P = F::P, D = 2 * HC;
   constexpr bool kF32 = sizeof(T) == 4;
   constexpr int TK = kF32 ? 1 : 2, STEP = 16 * TK, N = 4 * TK;  // score tiles, keys of a step and of a lane
   constexpr float kLift = kF32 ? 0.0f : F::kLift;
-  __shared__ float ml[2][4][16];
-  __shared__ f4 part[2][D][64];
+  __shared__ float ml[2][W][16];
+  __shared__ f4 part[W / 2][D][64];
   __shared__ uint32_t bad_rows;
   const int seq = blockIdx.y, per = a.heads / kv.nkv, hd = kv.hd;
   const int t0 = (blockIdx.x >> 3) % sl.few_tiles * kFewRows;  // the tile's first row
@@ -401,7 +403,7 @@ __global__ __launch_bounds__(256, HC <= 4 ? 3 : 1) void k_few(AttnArgs a, LayerV
   {
     const float *x = a.q + (size_t)(sp.q0 + tok) * a.q_stride + (size_t)head * hd;
     if constexpr (kF32) {
-      for (int c = wave; c < HC; c += 4) {
+      for (int c = wave; c < HC; c += W) {
         float v[8];
         query8(x, 32 * c + 8 * g, hd, vec, v);
 #pragma unroll
@@ -427,7 +429,7 @@ __global__ __launch_bounds__(256, HC <= 4 ? 3 : 1) void k_few(AttnArgs a, LayerV
           for (int i = 0; i < 8; ++i) v[c][i] = ldexpf(v[c][i], up);
         u4 q[P];
         F::parts(v[c], q);
-        if (c % 4 == wave)
+        if (c % W == wave)
 #pragma unroll
           for (int j = 0; j < P; ++j) ql[c][j][lane] = q[j];
       }
@@ -469,7 +471,7 @@ __global__ __launch_bounds__(256, HC <= 4 ? 3 : 1) void k_few(AttnArgs a, LayerV
         vr[d].zero();
     }
   };
-  constexpr int ALL = 4 * STEP;  // a step of every wave
+  constexpr int ALL = W * STEP;  // a step of every wave
   const int ko = N * (col >> 2), vo = N * g;
   int base = lo + STEP * wave, vpage = page_at(base + vo), knext = page_at(base + ALL + ko), vnext = page_at(base + ALL + vo);
   load_keys(base + ko, page_at(base + ko));
@@ -550,17 +552,17 @@ __global__ __launch_bounds__(256, HC <= 4 ? 3 : 1) void k_few(AttnArgs a, LayerV
     knext = page_at(base + 2 * ALL + ko);
     vnext = page_at(base + 2 * ALL + vo);
   }
-  // The four waves' softmaxes, then the four lane groups' shares of the sum.
+  // The waves' softmaxes, after the four lane groups' shares of the sum.
   l += __shfl_xor(l, 16);
   l += __shfl_xor(l, 32);
   if (g == 0) ml[0][wave][col] = m, ml[1][wave][col] = l;
   __syncthreads();
   float top = ml[0][0][col];
 #pragma unroll
-  for (int w = 1; w < 4; ++w) top = fmaxf(top, ml[0][w][col]);
+  for (int w = 1; w < W; ++w) top = fmaxf(top, ml[0][w][col]);
   float sum = 0.0f;
 #pragma unroll
-  for (int w = 0; w < 4; ++w) {
+  for (int w = 0; w < W; ++w) {
     const float mw = ml[0][w][col];
     sum += ml[1][w][col] * (mw == top ? 1.0f : __builtin_amdgcn_exp2f(mw - top));
   }
@@ -568,7 +570,7 @@ __global__ __launch_bounds__(256, HC <= 4 ? 3 : 1) void k_few(AttnArgs a, LayerV
 #pragma unroll
   for (int d = 0; d < D; ++d) o[d] *= mine;
 #pragma unroll
-  for (int from = 2; from; from >>= 1) {
+  for (int from = W / 2; from; from >>= 1) {
     if (wave >= from && wave < 2 * from)
 #pragma unroll
       for (int d = 0; d < D; ++d) part[wave - from][d][lane] = o[d];
@@ -609,7 +611,7 @@ __global__ __launch_bounds__(256, HC <= 4 ? 3 : 1) void k_few(AttnArgs a, LayerV
   }
   __syncthreads();
   if (bad_rows == 0) return;
-  for (int i = wave; i < rows; i += 4)
+  for (int i = wave; i < rows; i += W)
     if (bad_rows >> i & 1)
       redo_row(a, kv, table, sp.q0 + (t0 + i) / per, kvh * per + (t0 + i) % per, sp.n - sp.nq + (t0 + i) / per, lo, hi,
                sl.few, sl.few.at(row0 + i, split), splits > 1);
@@ -1035,13 +1037,13 @@ int many_split(size_t units, size_t tiles, int keys, int max_q, size_t row_bytes
 
 struct Plan {
   int few_len, many_len, few, many;  // split lengths and counts
-  int few_max, few_tiles;
+  int few_max, few_tiles, few_waves;
   size_t few_rows, many_rows, many_tiles;
   size_t few_parts() const { return few > 1 ? few * few_rows : 0; }
   size_t many_parts() const { return many > 1 ? many * many_rows : 0; }
 };
 
-Plan plan_of(int nkv, int heads, int hd, const BatchView &b, int window, size_t work_bytes) {
+Plan plan_of(int nkv, int heads, int hd, int size, const BatchView &b, int window, size_t work_bytes) {
   Plan p;
   const int per = heads / nkv, keys = most_keys(b, window);
   const size_t rows = (size_t)b.max_q * per, units = (size_t)b.seqs * nkv;
@@ -1065,7 +1067,12 @@ Plan plan_of(int nkv, int heads, int hd, const BatchView &b, int window, size_t 
   p.many_tiles = rows > (size_t)p.few_max ? (rows + kManyRows - 1) / kManyRows : 0;
   p.few = p.many = 1;
   p.few_len = p.many_len = std::max(256, whole128(keys));
-  if (p.few_tiles) {
+  // Few heads, short contexts: eight waves a block and no split while the join costs
+  // more than the one CU's time for the keys and values of a head, up to some 330 KB
+  // (one token, 32 heads, 8 waves against splits: 8 heads of 128 in f32, 300 positions
+  // 15 and 20 us, 500 21 and 20; 4 of 64 in bf16, 500 positions 9 and 13, 1000 13 and 14).
+  p.few_waves = hd <= 128 && units * p.few_tiles <= 256 && (size_t)keys * hd * size * 2 <= 330000 ? 8 : 4;
+  if (p.few_tiles && p.few_waves == 4) {
     const size_t want = std::max<size_t>(1, (b.seqs == 1 ? kFewBlocksOne : kFewBlocks) / (units * p.few_tiles));
     p.few_len = std::max(256, whole128(((size_t)keys + want - 1) / want));
     p.few = count(p.few_len, p.few_rows);
@@ -1087,21 +1094,25 @@ void launch_of(const AttnArgs &a, const LayerView<T> &kv, const BatchView &b, co
   }
   if (p.few_tiles) {
     const unsigned units = ((unsigned)p.few * kv.nkv + 7) / 8 * 8;
-    k_few<T, HC><<<dim3(units * p.few_tiles, b.seqs), 256, 0, s>>>(a, kv, b, sl, vec);
+    const dim3 grid(units * p.few_tiles, b.seqs);
+    if (HC <= 4 && p.few_waves == 8)
+      k_few<T, HC <= 4 ? HC : 4, 8><<<grid, 512, 0, s>>>(a, kv, b, sl, vec);
+    else
+      k_few<T, HC, 4><<<grid, 256, 0, s>>>(a, kv, b, sl, vec);
   }
 }
 
 }  // namespace
 
-size_t paged_attention_work(int nkv, int heads, int hd, const BatchView &b, int window) {
-  const Plan p = plan_of(nkv, heads, hd, b, window, SIZE_MAX);
+size_t paged_attention_work(int nkv, int heads, int hd, int size, const BatchView &b, int window) {
+  const Plan p = plan_of(nkv, heads, hd, size, b, window, SIZE_MAX);
   return (p.few_parts() + p.many_parts()) * (4 * (size_t)hd + 8);
 }
 
 template <class T>
 void launch_paged_attention(const AttnArgs &a, const LayerView<T> &kv, const BatchView &b, void *work,
                             size_t work_bytes, hipStream_t s) {
-  const Plan p = plan_of(kv.nkv, a.heads, kv.hd, b, a.window, work_bytes);
+  const Plan p = plan_of(kv.nkv, a.heads, kv.hd, (int)sizeof(T), b, a.window, work_bytes);
   Splits sl;
   sl.few_max = p.few_max;
   sl.few_tiles = p.few_tiles;
