@@ -364,7 +364,7 @@ __device__ __forceinline__ bool finite4(f4 x) {
 // gives the later ones the same keys.  32 sequences of up to 4096 positions, 32 heads on
 // 8 of 128 dimensions, bf16: 79 us, 4.5 TB/s; 9 tokens of 8 sequences, 16 heads, f32:
 // 77 us, 4.1 TB/s.  Short contexts of few heads are all latency, some 6 us and 1.5 to 2
-// a round of the waves: eight waves and no split there (launch_of).
+// a round of the waves: eight waves and no split there (plan_of).
 // HC: head size in steps of 32, rounded up; W: waves.
 template <class T, int HC, int W>
 __global__ __launch_bounds__(64 * W, W > 4 ? 2 : HC <= 4 ? 3 : 1) void k_few(AttnArgs a, LayerView<T> kv, BatchView b, Splits sl, bool vec) {
