@@ -403,7 +403,9 @@ int rai_paged_attention_dev(float *out, size_t out_stride, const float *q, size_
  * contents copied in all layers, and used[i] = 1 (else 0).  tables [seqs] and
  * tables_out [n] have rows of table_stride ids and must not overlap; the fresh pages
  * must be distinct and nobody's.  A parent outside 0..seqs-1: lengths_out 0, a table
- * row of -1.  Without a valid fresh[i] the entry becomes -1. */
+ * row of -1.  Without a valid fresh[i] the entry becomes -1.  Where the last page is
+ * not there (an id outside the pool) nothing is copied: the children keep the parent's
+ * entry, used[i] = 0. */
 int rai_paged_fork_dev(const rai_pages *pages, const int32_t *tables, size_t table_stride, const int32_t *lengths,
                        size_t seqs, const int32_t *parent, const int32_t *fresh, size_t n, int32_t *tables_out,
                        int32_t *lengths_out, int32_t *used, void *stream);

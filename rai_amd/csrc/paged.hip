@@ -263,8 +263,12 @@ __global__ __launch_bounds__(256) void k_fork(PoolBytes p, const int *tables, si
   int again = 0;
   for (int j = tid; j < i; j += 256) again |= parent[j] == par;
   again = __syncthreads_or(again);
-  const bool part = (len & ((1 << shift) - 1)) != 0, take = ok && part && again;
+  const bool part = (len & ((1 << shift) - 1)) != 0;
   const int last = len >> shift;  // the part-filled page's place
+  // A last page that is not there has nothing to copy: the fresh page, which holds what
+  // another sequence left in it, stays free, and the children name what the parent names.
+  const int src = ok && part && again ? tables[(size_t)par * stride + last] : -1;
+  const bool take = (unsigned)src < (unsigned)p.pages;
   if (!take || (unsigned)f >= (unsigned)p.pages) f = -1;
   if (blockIdx.x == 0) {
     for (size_t c = tid; c < stride; c += 256) {
@@ -278,8 +282,6 @@ __global__ __launch_bounds__(256) void k_fork(PoolBytes p, const int *tables, si
     }
   }
   if (f < 0) return;
-  const int src = tables[(size_t)par * stride + last];
-  if ((unsigned)src >= (unsigned)p.pages) return;
   copy_page(p, blockIdx.x / parts, src, f, blockIdx.x % parts);
 }
 

@@ -14,6 +14,23 @@ def pytest_configure(config):
     config.addinivalue_line("markers", "gpu: needs an MI355X (runs through the HIP library)")
 
 
+# Tests as they were written whose expected value contradicts the header, and why.  They run, and have to
+# fail (strict): what replaces them is named beside each.
+WRONG_VALUES = {
+    "test_gpu_paged.py::test_fork_bad_entries":
+        "expects the second child of a parent whose last page is not there to take a fresh page that nothing was "
+        "copied to: its attention would read what another sequence left in it "
+        "(test_fork_of_a_last_page_that_is_not_there; its other values: test_fork_lengths_past_the_table)",
+}
+
+
+def pytest_collection_modifyitems(items):
+    for item in items:
+        for name, why in WRONG_VALUES.items():
+            if item.nodeid.endswith(name):
+                item.add_marker(pytest.mark.xfail(reason=why, strict=True))
+
+
 @pytest.fixture(scope="session")
 def ora():
     """The CPU oracle (built on demand; test infrastructure only)."""

@@ -591,6 +591,66 @@ def test_fork_bad_entries(rai):
 
 
 @pytest.mark.parametrize("cache", CACHES)
+@pytest.mark.parametrize("missing", [-1, -3, "pages", 1 << 30])
+def test_fork_of_a_last_page_that_is_not_there(rai, cache, missing):
+    """No child sees a key there, and no fresh page is taken: it holds what another sequence left in it."""
+    heads, hd, lengths, parent = 4, 64, [40, 40, 21], np.int32([1, 0, 1, 0, 1, 2, 2])
+    n = len(parent)
+    pool = Pool(cache, 16, 2, hd, lengths, seed=9, layers=2, spare=n)
+    for layer in (0, 1):
+        pool.fill(layer, lengths)
+    for page in pool.spare:  # as another sequence left them
+        pool.tables[2, 2] = page
+        for layer in (0, 1):
+            for p in range(32, 48):
+                pool.put(layer, 2, p, *pool.rng.standard_normal((2, 2, hd)))
+    pool.tables[1, 2], pool.tables[2, 2] = pool.pages if missing == "pages" else missing, -1
+    dev = Dev(rai)
+    pg, fresh = dev.pages(pool), np.int32(pool.spare)
+    out = [dev.up(np.full(m, 77, np.int32)) for m in (3 * n, n, n)]
+    rai._check(rai.lib().rai_paged_fork_dev(pg, dev.up(pool.tables).ptr, 3, dev.up(np.int32(lengths)).ptr, 3,
+                                            dev.up(parent).ptr, dev.up(fresh).ptr, n, *[o.ptr for o in out], None))
+    rai._check(rai.lib().rai_device_synchronize())
+    tables, length, used = (o.to_host(np.int32, m) for o, m in zip(out, (3 * n, n, n)))
+    tables = tables.reshape(n, 3)
+    # Children 3 and 6 are the later ones of parents whose last page is there.
+    assert used.tolist() == [0, 0, 0, 1, 0, 0, 1] and length.tolist() == [lengths[p] for p in parent]
+    want = pool.tables[parent].copy()
+    want[3, 2], want[6, 1] = fresh[3], fresh[6]
+    assert np.array_equal(tables, want)
+    k, v = pool.k.copy(), pool.v.copy()
+    for child, last in ((3, 2), (6, 1)):
+        src = pool.tables[parent[child], last]
+        k[:, fresh[child]], v[:, fresh[child]] = pool.k[:, src], pool.v[:, src]
+    gk, gv = dev.pool_back(pool)
+    for got, copied in ((gk, k), (gv, v)):
+        assert np.array_equal(got.view(np.uint8), copied.view(np.uint8))
+    # Attention over a child is attention over its parent.
+    q = np.random.default_rng(1).standard_normal((n, heads, hd)).astype(np.float32)
+    opts = rai.AttentionOptions(hd ** -0.5, 0.0, 0, None)
+    batch = rai.PageBatch(out[0].ptr, 3, dev.up(np.int32(np.arange(n + 1))).ptr, out[1].ptr, n, n, 1, 40)
+    got = _run_attention(rai, dev, pg, batch, q, heads, hd, opts, layer=1)
+    for i, p in enumerate(parent):
+        ref, tol = attend(pool, 1, (i, 1, lengths[p]), p, q, heads, hd ** -0.5)
+        assert (np.abs(got[i] - ref[0]) <= tol[0]).all(), i
+
+
+def test_fork_lengths_past_the_table(rai):
+    """A length past the table becomes the table's: whole pages, shared by every child."""
+    pool = _random_pool("f32", 16, 1, 8, [40, 40], 2, 4)
+    dev = Dev(rai)
+    pg, parent, fresh = dev.pages(pool), np.int32([0, 0, 1, 0]), np.int32(pool.spare[:4])
+    out = [dev.up(np.zeros(m, np.int32)) for m in (12, 4, 4)]
+    rai._check(rai.lib().rai_paged_fork_dev(pg, dev.up(pool.tables).ptr, 3, dev.up(np.int32([10 ** 9, -5])).ptr, 2,
+                                            dev.up(parent).ptr, dev.up(fresh).ptr, 4, *[o.ptr for o in out], None))
+    rai._check(rai.lib().rai_device_synchronize())
+    assert out[1].to_host(np.int32, 4).tolist() == [48, 48, 0, 48] and not out[2].to_host(np.int32, 4).any()
+    assert np.array_equal(out[0].to_host(np.int32, 12).reshape(4, 3), pool.tables[parent])
+    gk, gv = dev.pool_back(pool)
+    assert np.array_equal(gk, pool.k) and np.array_equal(gv, pool.v)
+
+
+@pytest.mark.parametrize("cache", CACHES)
 @pytest.mark.parametrize("page,kv_heads,hd,layers,n,entries", [(16, 1, 8, 1, 1, 0), (64, 2, 128, 2, 9, 40),
                                                               (32, 3, 72, 3, 300, 5000)])
 def test_move(rai, cache, page, kv_heads, hd, layers, n, entries):
