@@ -139,3 +139,44 @@ def attend(pool, layer, span, seq, q, heads, scale, softcap=0.0, window=0, slope
             worst = (p * np.expm1(np.minimum(2 * (off + off.max()), 50.0))) @ np.abs(vv)
             tol[j, h] = worst + EPS32 * (len(seen) + 16) * (p @ np.abs(vv)) + EPS32 * (p @ np.abs(vv))
     return out, tol
+
+
+# How far normal inputs' attention may be off in f32, in half steps of the 2-norm.  A score's sum of hd products
+# passes through at most 96 f32 sums (hd 256 in sixteenths, six products each), the output's through 57 per 300 keys
+# of a block's share and part; a rounding is off by at most two half steps (one when to nearest) of a partial sum
+# that is 0.7 of the result in the mean square.  Independent ones add up as squares: 0.7 * 2 * sqrt(96) = 14 for the
+# score, 0.7 * 2 * sqrt(3 * 57) / sqrt(3) = 11 for the output, 5 for the exponential and its argument: 18, and
+# dividing, joining and the operands' last bits (2) are within 25.  A row by itself, few of whose weights may carry
+# it: twice that.
+ACCURATE = 25
+
+
+def off_by(got, want):
+    """Half steps of the 2-norm: all rows [..][hd] together, and the worst row."""
+    d = np.linalg.norm(got.astype(np.float64) - want, axis=-1)
+    n = np.linalg.norm(want, axis=-1)
+    return np.linalg.norm(d) / np.linalg.norm(n) / EPS32, (d / n).max() / EPS32
+
+
+def cut(x, cache, parts):
+    """f32 values as the parts that a 16-bit matrix operand holds, largest first: bf16 parts cut off, f16 parts
+    rounded."""
+    out, rest = [], np.array(x, np.float32)
+    for _ in range(parts):
+        if cache == "f16":
+            h = rest.astype(np.float16).astype(np.float32)
+        else:
+            h = (rest.view(np.uint32) & np.uint32(0xFFFF0000)).view(np.float32)
+        out.append(h.astype(np.float64))
+        rest = rest - h
+    return out
+
+
+def attend_cut(q, k, v, cache, query_parts, weight_parts, key_parts=1, value_parts=1, products=None):
+    """softmax(q k^T / sqrt(hd)) v in f64 whose operands are cut into parts, of whose pairs i + j < products count."""
+    def dot(a, b, m):
+        return sum(x @ y for i, x in enumerate(a) for j, y in enumerate(b) if i + j < (products or len(a) + m))
+
+    s = dot(cut(q, cache, query_parts), [x.T for x in cut(k, cache, key_parts)], key_parts) / np.sqrt(q.shape[1])
+    p = np.exp(s - s.max(1, keepdims=True))
+    return dot(cut(p * 2.0 ** 14, cache, weight_parts), cut(v, cache, value_parts), value_parts) / 2.0 ** 14 / p.sum(1, keepdims=True)

@@ -9,6 +9,7 @@ import numpy as np
 import pytest
 
 from conftest import ROOT
+from paged_model import ACCURATE, attend_cut, decode, encode, off_by
 
 P = ctypes.c_void_p
 AT = 4096  # an aligned address that no refused call reads
@@ -221,3 +222,21 @@ def test_index_bounds(tmp_path):
                     "-I", os.path.join(ROOT, "rai_amd", "csrc"), os.path.join(ROOT, "tests", "paged_index_check.cpp"),
                     "-o", exe], check=True)
     assert subprocess.run([exe], capture_output=True, text=True, check=True).stdout == "ok\n"
+
+
+@pytest.mark.parametrize("cache", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("hd", [64, 128, 256])
+def test_parts_of_matrix_operands(cache, hd):
+    """The parts that the attention's 16-bit operands are cut into leave f32 accuracy; with a part less in any
+    operand, or fewer products, attention is off by several times what its tests on the GPU allow."""
+    r = np.random.default_rng(hd)
+    q = r.standard_normal((32, hd)).astype(np.float32)
+    k, v = (decode(encode(r.standard_normal((900, hd)), cache), cache) for _ in range(2))
+    s = q.astype(np.float64) @ k.T.astype(np.float64) / np.sqrt(hd)
+    p = np.exp(s - s.max(1, keepdims=True))
+    want = p @ v.astype(np.float64) / p.sum(1, keepdims=True)
+    whole = {"f32": dict(query_parts=3, weight_parts=3, key_parts=3, value_parts=3, products=3),
+             "f16": dict(query_parts=2, weight_parts=2), "bf16": dict(query_parts=3, weight_parts=3)}[cache]
+    assert off_by(attend_cut(q, k, v, cache, **whole), want)[0] < 3
+    for name, n in whole.items():
+        assert off_by(attend_cut(q, k, v, cache, **{**whole, name: n - 1}), want)[0] > 4 * ACCURATE, name

@@ -7,7 +7,7 @@ import gc
 import numpy as np
 import pytest
 
-from paged_model import EPS32, Pool, attend, decode, encode, rotate, spans, store_dtype
+from paged_model import ACCURATE, EPS32, Pool, attend, decode, encode, off_by, rotate, spans, store_dtype
 
 pytestmark = pytest.mark.gpu
 
@@ -242,6 +242,27 @@ def test_attention_random_batches(rai, seed):
                      softcap=float(r.choice([0.0, 3.0, 25.0])), window=int(r.choice([0, 1, 7, 64, 301])), slopes=slopes,
                      front=int(r.integers(3)), back=int(r.integers(3)), layer=1, ld=int(heads * hd + r.choice([0, 1, 4])),
                      out_ld=int(heads * hd + r.choice([0, 3, 4])), works=(None, 0, int(4096 * r.integers(1, 40))))
+
+
+@pytest.mark.parametrize("cache", CACHES)
+@pytest.mark.parametrize("hd", [64, 128, 256])
+@pytest.mark.parametrize("news,lengths,split", [([1, 1], [200, 180], False), ([1, 3], [2000, 900], False),
+                                                ([1, 3], [2000, 900], True), ([90], [700], False), ([90], [1800], True)])
+def test_attention_is_as_accurate_as_f32(rai, cache, hd, news, lengths, split):
+    """Normal inputs, by norms: few rows and chunks, in one pass and in splits."""
+    heads, kv_heads, tokens = 4, 2, sum(news)
+    pool = Pool(cache, 32, kv_heads, hd, lengths, seed=hd + tokens)
+    pool.fill(0, lengths)
+    q = np.random.default_rng(hd).standard_normal((tokens, heads, hd)).astype(np.float32)
+    dev, starts = Dev(rai), _starts(news)
+    pg, batch = dev.pages(pool), dev.batch(pool, starts, lengths, tokens, max(news), max(lengths))
+    opts = rai.AttentionOptions(hd ** -0.5, 0.0, 0, None)
+    assert not split or rai.attention_workspace(heads, pg, batch, opts) > 0
+    got = _run_attention(rai, dev, pg, batch, q, heads, hd, opts, work=None if split else 0)
+    want = np.concatenate([attend(pool, 0, (int(a), m, n), s, q, heads, hd ** -0.5)[0]
+                           for s, (a, m, n) in enumerate(zip(starts, news, lengths))])
+    total, row = off_by(got, want)
+    assert total <= ACCURATE and row <= 2 * ACCURATE, (total, row)
 
 
 def test_attention_calls_on_two_streams_and_in_a_graph(rai):
