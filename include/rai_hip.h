@@ -405,7 +405,8 @@ int rai_paged_attention_dev(float *out, size_t out_stride, const float *q, size_
  * must be distinct and nobody's.  A parent outside 0..seqs-1: lengths_out 0, a table
  * row of -1.  Without a valid fresh[i] the entry becomes -1.  Where the last page is
  * not there (an id outside the pool) nothing is copied: the children keep the parent's
- * entry, used[i] = 0. */
+ * entry, used[i] = 0.  At most 65535 parents and children a call, and layers x the parts
+ * of 32 KB that a page's keys in one layer have at most 2^23. */
 int rai_paged_fork_dev(const rai_pages *pages, const int32_t *tables, size_t table_stride, const int32_t *lengths,
                        size_t seqs, const int32_t *parent, const int32_t *fresh, size_t n, int32_t *tables_out,
                        int32_t *lengths_out, int32_t *used, void *stream);
@@ -413,7 +414,9 @@ int rai_paged_fork_dev(const rai_pages *pages, const int32_t *tables, size_t tab
 /* Moves n pages: page src[i] is copied to dst[i] in all layers, and each of the
  * `entries` ids of `tables` (may be NULL) that names src[i] names dst[i] afterwards.
  * src are distinct, dst are distinct and none of src (a copy goes to a free page).
- * Pairs with an id outside the pool are left out. */
+ * Pairs with an id outside the pool are left out.  At most 65535 pages a call, and pages
+ * x layers x the parts of 32 KB that a page's keys in one layer have below 2^23 (512 GB
+ * of full parts). */
 int rai_paged_move_dev(const rai_pages *pages, const int32_t *src, const int32_t *dst, size_t n, int32_t *tables,
                        size_t entries, void *stream);
 

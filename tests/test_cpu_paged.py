@@ -141,6 +141,18 @@ def test_refused_forks_and_moves(rai):
     assert L.rai_paged_move_dev(pg, None, None, 0, None, 0, None) == 0
 
 
+def test_limits_of_forks_and_moves(rai):
+    """Pages x layers of a launch, in parts of 32 KB: of 2 KB (one part) and of 64 MB pages (2048)."""
+    L, small, large = rai.lib(), dict(page_size=16, kv_heads=1, head_dim=32), dict(page_size=1024, kv_heads=64, head_dim=256)
+    for n, layers, kw in [(65535, 129, small), (1, 4096, large), (2, 2048, large)]:
+        _refused(rai, L.rai_paged_move_dev(_pages(rai, layers=layers, **kw), AT, AT, n, None, 0, None), "RAI_E_SHAPE",
+                 "pages x layers")
+    _refused(rai, L.rai_paged_fork_dev(_pages(rai, layers=4097, **large), AT, 4, AT, 2, AT, AT, 2, 2 * AT, 2 * AT, AT, None),
+             "RAI_E_SHAPE", "overflow")
+    _refused(rai, L.rai_paged_fork_dev(_pages(rai), AT, 4, AT, 65536, AT, AT, 2, 2 * AT, 2 * AT, AT, None), "RAI_E_SHAPE",
+             "65535")
+
+
 def test_refused_selections(rai):
     L, need = rai.lib(), rai.beam_workspace(100, 2, 3, 6)
     good = [AT, 100, 100, AT, AT, 5, 2, 3, 6, AT, AT, AT, AT, need, None]

@@ -696,6 +696,43 @@ def test_move(rai, cache, page, kv_heads, hd, layers, n, entries):
         assert dt.to_host(np.int32, entries).tolist() == [name.get(t, t) for t in tables]
 
 
+@pytest.mark.parametrize("n,entries", [(2100, 70001), (4096, 65536), (65535, 3)])
+def test_move_many(rai, n, entries):
+    """More pairs than are looked through in one go, more table entries than the launch has threads."""
+    pool = _random_pool("f16", 16, 1, 8, [1], 1, 2 * n + 8)
+    r = np.random.default_rng(n)
+    ids = r.permutation(pool.pages).astype(np.int32)
+    src, dst = ids[:n].copy(), ids[n:2 * n].copy()
+    src[n // 2], dst[n - 2] = pool.pages, -1  # left out
+    tables = r.integers(-2, pool.pages + 2, entries).astype(np.int32)
+    tables[-3:] = src[0], src[n - 1], src[n - 2]
+    dev = Dev(rai)
+    pg, dt = dev.pages(pool), dev.up(tables)
+    rai._check(rai.lib().rai_paged_move_dev(pg, dev.up(src).ptr, dev.up(dst).ptr, n, dt.ptr, entries, None))
+    rai._check(rai.lib().rai_device_synchronize())
+    ok = (src < pool.pages) & (dst >= 0)
+    k, v, name = pool.k.copy(), pool.v.copy(), np.arange(-2, pool.pages + 2)
+    k[:, dst[ok]], v[:, dst[ok]], name[src[ok] + 2] = pool.k[:, src[ok]], pool.v[:, src[ok]], dst[ok]
+    gk, gv = dev.pool_back(pool)
+    assert np.array_equal(gk.view(np.uint16), k.view(np.uint16)) and np.array_equal(gv.view(np.uint16), v.view(np.uint16))
+    assert np.array_equal(dt.to_host(np.int32, entries), name[tables + 2])
+
+
+def test_move_of_the_largest_launch(rai):
+    """65535 pairs x 128 layers, one below the limit of pages x layers; all but the first and last left out."""
+    n, pool = 65535, _random_pool("f16", 16, 1, 8, [1], 128, 7)
+    src, dst = np.full(n, -1, np.int32), np.full(n, -1, np.int32)
+    (src[0], src[-1]), (dst[0], dst[-1]) = pool.spare[:2], pool.spare[2:4]
+    dev = Dev(rai)
+    pg = dev.pages(pool)
+    rai._check(rai.lib().rai_paged_move_dev(pg, dev.up(src).ptr, dev.up(dst).ptr, n, None, 0, None))
+    rai._check(rai.lib().rai_device_synchronize())
+    k, v = pool.k.copy(), pool.v.copy()
+    k[:, pool.spare[2:4]], v[:, pool.spare[2:4]] = pool.k[:, pool.spare[:2]], pool.v[:, pool.spare[:2]]
+    gk, gv = dev.pool_back(pool)
+    assert np.array_equal(gk.view(np.uint16), k.view(np.uint16)) and np.array_equal(gv.view(np.uint16), v.view(np.uint16))
+
+
 # -------------------------------------------------------------------- beam --
 
 def _select(x, scores, done, end, beams, take):
@@ -761,6 +798,23 @@ def test_beam(rai, groups, beams, vocab, take, extra):
     r = np.random.default_rng(vocab + take)
     x = _normal(r, groups * beams, vocab, 2.5)
     _check_beam(rai, x, -np.abs(3 * r.standard_normal(groups * beams)), None, 0, beams, take, extra)
+
+
+@pytest.mark.parametrize("best", ["spread", "last beams", "one chunk"])
+@pytest.mark.parametrize("take", [7, 64])
+def test_beam_many_lists(rai, best, take):
+    """64 beams of 38 chunks: more lists than the merge looks at in one go, so that the first places of some come
+    after later places of others."""
+    r = np.random.default_rng(take)
+    vocab = 151936
+    x = _normal(r, 64, vocab, 2.0)
+    scores = -np.abs(3 * r.standard_normal(64))
+    if best == "last beams":
+        scores[:] = np.linspace(-40, -1, 64)
+    if best == "one chunk":  # the best are the later places of the last list, behind everything else's first
+        scores[:] = np.linspace(-9, -8, 64)
+        x[63, vocab - 300:vocab - 300 + 2 * 80:2] = 14.0 + 0.01 * r.permutation(80)
+    _check_beam(rai, x, scores, None, 0, 64, take)
 
 
 @pytest.mark.parametrize("vocab,take", [(5, 8), (1000, 8), (20000, 20)])
