@@ -347,8 +347,8 @@ typedef enum rai_rope_scaling {
   RAI_ROPE_LINEAR = 1, /* every frequency divided by factor */
   RAI_ROPE_LLAMA3 = 2, /* those that turn less than low_freq times over trained_context divided, those
                           that turn more than high_freq times kept, blended between */
-  RAI_ROPE_YARN = 3    /* the same blended by pair index (low_freq, high_freq: 1 and 32 turns), and
-                          the gain 0.1 ln(factor) + 1 */
+  RAI_ROPE_YARN = 3    /* the same blended by pair index, between the pairs that turn once and 32 times
+                          (low_freq and high_freq are not read), and the gain 0.1 ln(factor) + 1 */
 } rai_rope_scaling;
 
 /* Host only: the inverse frequencies theta^(-2i / rot_dim), i < rot_dim / 2, under
@@ -382,7 +382,9 @@ typedef struct rai_attention_options {
 /* Causal attention of the batch's rows over `layer` of their sequences' pages
  * (keys and values of the rows themselves are in the pages: rai_paged_store_dev
  * first): out row = sum_j softmax_j(score) v_j over the positions it sees, heads /
- * kv_heads query heads on each kv head.  f32 accuracy for every cache type.  A row
+ * kv_heads query heads on each kv head.  f32 accuracy for every cache type; over an f16
+ * cache a query row's elements and its keys' weights are held to 2^-22 of themselves, or to
+ * 2^-39 of the row's largest where that is more.  A row
  * that sees nothing, or only scores of -inf, becomes zeros.  out must not overlap q; tokens * heads is at most
  * 2^24 - 1.  What a row does not see does not reach it,
  * NaN and infinities included.
@@ -426,7 +428,9 @@ int rai_paged_move_dev(const rai_pages *pages, const int32_t *src, const int32_t
  * group * beams + beam, what rai_paged_fork_dev takes), token and score
  * [groups][take], best first, equal ones by beam, then logit, then token.  done (may be NULL)
  * [groups * beams]: a finished beam's only candidate is end_token at its present
- * score.  Scores are summed and compared in f64.  NaN logits count as -inf; a row
+ * score.  Scores are summed and compared in f64; the exponentials of a row's log-sum are
+ * f32 ones, which leaves it within 2e-6 (some 1e-8 as a rule): candidates of different
+ * beams that are nearer than that may come in either order.  NaN logits count as -inf; a row
  * without a finite log-sum (all -inf, or +inf) and beams whose score is not finite
  * have no candidates, and neither has a token at -inf; places past the last candidate
  * become -1, -1, -inf.  beams <= 64, take <= 64, groups * beams <= 65535,

@@ -298,7 +298,8 @@ class DeviceArray:
 
 def rope_frequencies(scaling: int, theta: float, rot_dim: int, factor: float = 1.0, trained_context: float = 8192.0,
                      low_freq: float = 1.0, high_freq: float = 4.0) -> tuple[np.ndarray, float]:
-    """rai_rope_frequencies: (inverse frequencies [rot_dim / 2] in f64, gain) of a rotary scaling."""
+    """rai_rope_frequencies: (inverse frequencies [rot_dim / 2] in f64, gain) of a rotary scaling (low_freq and
+    high_freq: of ROPE_LLAMA3 alone)."""
     inv, gain = np.zeros(rot_dim // 2, np.float64), c_float()
     _check(lib().rai_rope_frequencies(scaling, theta, rot_dim, factor, trained_context, low_freq, high_freq,
                                       _ptr(inv), ctypes.byref(gain)))

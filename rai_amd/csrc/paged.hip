@@ -33,8 +33,8 @@ struct StoreArgs {
 // cos and sin of pos * inv, both times gain.  The angle and its reduction to a
 // quarter turn and f, -1/2..1/2 of one, in f64 (an f32 angle of a far position is
 // off by more than the rotation may be); sin and cos of f quarter turns as
-// polynomials in f^2 with the smallest relative error (3e-9 and 6e-11, so f32's own
-// rounding is what is left).
+// polynomials in f^2 with the smallest relative error (with coefficients rounded to f32
+// 3.4e-8 and 8e-9, a half step of f32 being 6e-8; evaluated in f32 1.3e-7 and 8e-8).
 __device__ __forceinline__ void rope_angle(int pos, double inv, float gain, float &c, float &s) {
   const double a = (double)pos * (inv * 0.63661977236758138);
   const double n = rint(a);

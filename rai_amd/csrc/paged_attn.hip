@@ -9,10 +9,11 @@
 //
 // f32 accuracy from 16-bit operands.  An f32 value is the exact sum of three bf16
 // ones (8 + 8 + 8 bits, each cut off), so a product with a bf16 value is three
-// exact products, and one of two f32 values the six of nine whose weight reaches
-// 2^-24.  Against f16 values two f16 parts do (11 + 11 bits and the sign of the
-// second), the queries of a row scaled by a power of two so that the range of f16
-// cannot cut them, the probabilities by 2^14.  The f32 matrix instructions run at
+// exact products, and one of two f32 values the six largest of nine: the others are
+// below 2^-21 of it together, 1.8 half steps of f32 in a normal row's result.  Against f16
+// values two f16 parts do (11 + 11 bits and the sign of the second), the queries of a
+// row scaled by a power of two that brings the largest to 2^14 .. 2^15, the
+// probabilities by 2^14: what is below 2^-17 of the largest has fewer bits, to 2^-39 of it.  The f32 matrix instructions run at
 // a sixteenth of the 16-bit rate: three or six products are the faster way.
 //
 // Layout.  The instruction leaves row 4 g + i (16 x 16) or 8 b + 4 h + c (32 x 32)
@@ -54,7 +55,7 @@ __device__ __forceinline__ float wave_sum(float x) {
 }
 
 // tanh.  Near zero, where 1 - 2 / (e^2x + 1) cancels, x + x^3 P(x^2) with P fitted to
-// the smallest relative error over 0..0.625 (4e-9).
+// the smallest relative error over 0..0.625 (6e-9).
 constexpr float kTanhNear = 0.625f;
 __device__ __forceinline__ float tanh_near(float x) {
   const float y = x * x;
@@ -362,7 +363,7 @@ __device__ __forceinline__ bool finite4(f4 x) {
 // times as fast as memory delivers; cutting the values took some 700 vector instructions
 // a step).  The tiles of one split run side by side on one XCD (blocks 8 apart), whose L2
 // gives the later ones the same keys.  32 sequences of up to 4096 positions, 32 heads on
-// 8 of 128 dimensions, bf16: 79 us, 4.5 TB/s; 9 tokens of 8 sequences, 16 heads, f32:
+// 8 of 128 dimensions, bf16: 79 us, 4.4 TB/s; 9 tokens of 8 sequences, 16 heads, f32:
 // 77 us, 4.1 TB/s.  Short contexts of few heads are all latency, some 6 us and 1.5 to 2
 // a round of the waves: eight waves and no split there (plan_of).
 // HC: head size in steps of 32, rounded up; W: waves.

@@ -265,6 +265,39 @@ def test_attention_is_as_accurate_as_f32(rai, cache, hd, news, lengths, split):
     assert total <= ACCURATE and row <= 2 * ACCURATE, (total, row)
 
 
+@pytest.mark.parametrize("cache", CACHES)
+@pytest.mark.parametrize("nq", [1, 40])
+def test_attention_of_a_wide_range(rai, cache, nq):
+    """A query element of 2^30 that meets zeros beside normal ones, and a key of weight 2^-29 that alone has
+    values in one dimension: f32's accuracy, or with f16 what the header says."""
+    heads, hd, n, scale = 4, 64, 200, 0.125
+    pool = Pool(cache, 16, 1, hd, [n], seed=12)
+    pool.fill(0, [n])
+    q = np.random.default_rng(3).standard_normal((nq, heads, hd)).astype(np.float32)
+    q[:, :, 5], q[:, :, 9] = 2.0 ** 30, 8.0
+    for p in range(n):
+        pg, slot = pool.place(0, p)
+        pool.k[0, pg, :, slot, 5] = encode(np.float32([0.0]), cache)[0]
+        pool.v[0, pg, :, 7, slot] = encode(np.float32([1.0 if p == 3 else 0.0]), cache)[0]
+        pool.k[0, pg, :, slot, 9] = encode(np.float32([-20.0 if p == 3 else 0.0]), cache)[0]
+    want, tol = attend(pool, 0, (0, nq, n), 0, q, heads, scale)
+    if cache == "f16":
+        k, v, _ = pool.rows(0, 0, np.arange(n))
+        for j in range(nq):
+            seen = n - nq + j + 1
+            kk, vv = np.abs(k[:seen, 0]), np.abs(v[:seen, 0])
+            for h in range(heads):
+                s = k[:seen, 0] @ q[j, h].astype(np.float64) * scale
+                w = np.exp(s - s.max())
+                x = np.abs(q[j, h].astype(np.float64))
+                off = kk @ np.maximum(2.0 ** -22 * x, 2.0 ** -39 * x.max()) * scale
+                tol[j, h] += (w / w.sum() * np.expm1(2 * off.max())) @ vv + np.maximum(2.0 ** -22 * w, 2.0 ** -39) / w.sum() @ vv
+    dev = Dev(rai)
+    pg, batch = dev.pages(pool), dev.batch(pool, [0, nq], [n], nq, nq, n)
+    got = _run_attention(rai, dev, pg, batch, q, heads, hd, rai.AttentionOptions(scale, 0.0, 0, None))
+    assert (np.abs(got - want) <= tol).all()
+
+
 def test_attention_calls_on_two_streams_and_in_a_graph(rai):
     """Two calls in flight with scratch of their own; a captured call replayed on new lengths and queries."""
     L, P, heads, hd = rai.lib(), ctypes.c_void_p, 8, 64
