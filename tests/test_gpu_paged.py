@@ -1031,6 +1031,58 @@ def test_a_step_in_a_graph(rai):
 
 
 @pytest.mark.parametrize("cache", CACHES)
+def test_an_attention_block_of_the_framework_s_calls(rai, ora, cache):
+    """Norm, fused W4A8 projection, store (queries turned in place, in the projection's rows), attention and
+    output projection on one stream, over two layers of pages: each stage from what the one before left."""
+    from rai_amd.workload import gemv_operands
+    L, heads, kv_heads, hd, gs, wide = rai.lib(), 4, 2, 64, 64, 256
+    news, lengths, rows = [1, 9, 2], [40, 29, 2], (4 + 2 * 2) * 64
+    tokens, starts = sum(news), _starts(news)
+    pool = Pool(cache, 16, kv_heads, hd, lengths, seed=13, layers=2)
+    for layer in (0, 1):
+        pool.fill(layer, [n - m for m, n in zip(news, lengths)])
+    dev, r = Dev(rai), np.random.default_rng(7)
+    pg, batch = dev.pages(pool), dev.batch(pool, starts, lengths, tokens, max(news), max(lengths))
+    inv, gain = rai.rope_frequencies(rai.ROPE_LLAMA3, 1e4, hd, 8.0, 32.0)
+    rope, opts = rai.Rope(dev.up(inv).ptr, hd, 0, gain), rai.AttentionOptions(hd ** -0.5, 0.0, 0, None)
+    x, weight = r.standard_normal((tokens, wide)).astype(np.float32), r.standard_normal(wide).astype(np.float32)
+    need = rai.attention_workspace(heads, pg, batch, opts)
+    dw, dx, dg = rai.DeviceArray(max(need, 16)), dev.up(x), dev.up(weight)
+    for layer in (0, 1):
+        qkv, proj = (gemv_operands(a, wide, 1, gs, seed=layer + a)[:2] for a in (rows, wide))
+        dy, dq, da, do = (rai.DeviceArray(4 * tokens * n) for n in (wide, rows, wide, wide))
+        base = dq.ptr
+        weights = [dev.up(a).ptr for a in (*qkv, *proj)]
+        rcs = [L.rai_rms_norm_dev(dy.ptr, dx.ptr, dg.ptr, tokens, wide, 1e-5, None),
+               L.rai_w4a8_matmul_dev(dq.ptr, weights[0], weights[1], dy.ptr, rows, wide, tokens, gs, None)]
+        rai._check(L.rai_device_synchronize())
+        before = dq.to_host(np.float32, tokens * rows).reshape(tokens, rows)
+        rcs += [L.rai_paged_store_dev(pg, layer, batch, rope, base, rows, base, rows, heads, base + 4 * heads * hd, rows,
+                                      base + 4 * (heads + kv_heads) * hd, rows, None),
+                L.rai_paged_attention_dev(da.ptr, wide, base, rows, heads, pg, layer, batch, opts, dw.ptr, need, None),
+                L.rai_w4a8_matmul_dev(do.ptr, weights[2], weights[3], da.ptr, wide, wide, tokens, gs, None)]
+        assert rcs == [0] * 5, L.rai_last_error()
+        rai._check(L.rai_device_synchronize())
+        y, after, att, out = (a.to_host(np.float32, tokens * n).reshape(tokens, n)
+                              for a, n in ((dy, wide), (dq, rows), (da, wide), (do, wide)))
+        assert np.array_equal(before.reshape(-1), ora.w4a8_matmul(*qkv, y, rows, wide, tokens, gs).reshape(-1))
+        assert np.array_equal(out.reshape(-1), ora.w4a8_matmul(*proj, att, wide, wide, tokens, gs).reshape(-1))
+        assert np.array_equal(after[:, heads * hd:], before[:, heads * hd:])
+        pool.k[:], pool.v[:] = dev.pool_back(pool)
+        for s, (a, m, n) in enumerate(zip(starts, news, lengths)):
+            for j in range(m):
+                q = before[a + j, :heads * hd].reshape(heads, hd)
+                # Two products, a sum and the angle's cosine and sine, each within three half steps.
+                size = 8 * EPS32 * gain * np.sqrt(2) * np.abs(before[a + j]).max()
+                want = rotate(q, n - m + j, inv, hd, 0, gain)
+                assert (np.abs(after[a + j, :heads * hd].reshape(heads, hd) - want) <= size).all()
+            q = after[:, :heads * hd].reshape(tokens, heads, hd)
+            want, tol = attend(pool, layer, (int(a), m, n), s, q, heads, hd ** -0.5)
+            assert (np.abs(att[a:a + m].reshape(m, heads, hd) - want) <= tol).all()
+        dx = do
+
+
+@pytest.mark.parametrize("cache", CACHES)
 def test_beam_search_over_the_pages(rai, cache):
     """A beam search as a program runs it: the prompt stored and attended as a chunk, then steps of
     selection, fork, store and attention; every step's attention equals attention over each beam's own
