@@ -429,7 +429,7 @@ int rai_paged_move_dev(const rai_pages *pages, const int32_t *src, const int32_t
  * [groups][take], best first, equal ones by beam, then logit, then token.  done (may be NULL)
  * [groups * beams]: a finished beam's only candidate is end_token at its present
  * score.  Scores are summed and compared in f64; the exponentials of a row's log-sum are
- * f32 ones, which leaves it within 2e-6 (some 1e-8 as a rule): candidates of different
+ * f32 ones, which leaves it within 3e-6 (some 1e-8 as a rule): candidates of different
  * beams that are nearer than that may come in either order.  NaN logits count as -inf; a row
  * without a finite log-sum (all -inf, or +inf) and beams whose score is not finite
  * have no candidates, and neither has a token at -inf; places past the last candidate

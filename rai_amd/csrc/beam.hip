@@ -50,8 +50,8 @@ __device__ __forceinline__ float logit_of(uint64_t k) {
 
 // exp(x - top), x <= top: the product with log2 e carries its rounding along, so
 // that only the half steps of the difference and of the exponential are left.  A
-// row's log-sum: a half step of a difference of up to log(vocab) in the mean, two of the
-// exponential, one of the correction, 15 of a thread's sum, 2e-6 together.
+// row's log-sum: half steps of a difference of up to log(vocab), 21, in the mean, two of
+// the exponential, one of the correction, 15 of a thread's sum: 3e-6 together at most.
 __device__ __forceinline__ float exp_near(float x, float top) {
   constexpr float kLog2e = 1.4426950408889634f, kLow = 1.9259629911266175e-8f, kLn2 = 0.6931471805599453f;
   const float d = fmaxf(x - top, -200.0f), t = d * kLog2e;
